@@ -194,7 +194,7 @@ def _own(st):
     out = {n: st[n] for n in ("logprob", "entropy")}
     if case["kind"] == "nll":
         ctx.token_logprobs_grad(st["logits"], st["tokens"], st["g_logprob"], None, st["logprob"], st["entropy"],
-                                st["stats"], st["d_logits"], M, V, act)
+                                st["stats"], st["d_logits"], M, V, act, st["ws"])
         return dict(out, d_logits=st["d_logits"])
     ctx.token_logprobs(st["logits"], st["tokens"], st["logprob"], st["entropy"], st["stats"], st["top_ids"],
                        st["top_logprobs"], M, V, k, act, st["ws"])
