@@ -32,8 +32,8 @@
  * graphs may be replayed on any stream, beside other work of the context and
  * after it is destroyed.  Exceptions: lssm_ssd_chunked holds workspaces of the
  * context (replays must be ordered with its other scans, and the context must
- * outlive the graph); lssm_embed and the fused batch-1 entries hold its status
- * word (it must outlive the graph); and what the entries below state.
+ * outlive the graph); lssm_embed, lssm_token_logprobs and the fused batch-1
+ * entries hold its status word (it must outlive the graph); and what the entries below state.
  * Captured, lssm_linear runs with K unsplit where it otherwise splits it over
  * several blocks (the same products, summed in another order), and
  * lssm_norm_linear_decode and lssm_inproj_decode normalise their rows again in
@@ -139,6 +139,8 @@ int lssm_sync(lssm_ctx* ctx);              /* stream sync + error check         
  *     in_proj epilogue, before any wait), so the step must not be retried on
  *     the same state.
  *   Both conditions in one step report LSSM_EINVAL with both texts.
+ *   - a token to score is not below the vocabulary (lssm_token_logprobs):
+ *     LSSM_EINVAL, "token_logprobs: a token is not below the vocabulary".
  *
  * Failure-injection switches for the tests of these paths (no counterpart in
  * the reference; 0 = off, the default).  LSSM_DEBUG_STALE_WAIT makes the SSD
@@ -383,6 +385,54 @@ int lssm_embed(lssm_ctx* ctx, const void* table, const int32_t* ids, void* out,
 /* ids[r] = first index of the max of logits[r, :]  (sampler.cpp:13-21). */
 int lssm_argmax(lssm_ctx* ctx, const void* logits, int32_t* ids, uint32_t rows,
                 uint32_t vocab, lssm_dtype act);
+
+/* Log probabilities under rows of logits [rows, vocab] (row stride in elements,
+ * 0 = packed), held in 32 bits throughout.  Per row, with m the largest logit
+ * and ls = log sum e^(x - m):
+ *   logprob  [rows]       log p(tokens[r]) = (x_t - m) - ls; 0 where tokens[r] is
+ *                         negative (a position without a token to score)
+ *   entropy  [rows]       -sum p log p, in nats
+ *   stats    [rows, 2]    m and ls, as lssm_token_logprobs_bwd takes them
+ *   top_ids, top_logprobs [rows, top_k]  the top_k likeliest tokens, likeliest
+ *                         first, of equal ones the lowest id first
+ * logprob (then tokens too), entropy and stats may be NULL.  A masked logit
+ * (-inf) has probability 0 and is no alternative; places left over hold id -1
+ * and -inf.  A row with nothing but -inf has log probability -inf, entropy 0,
+ * stats (0, inf) and a zero gradient.  A row that holds a NaN or +inf is NaN.  A
+ * token that is not below vocab gives NaN and is reported at the next
+ * synchronisation point (LSSM_EINVAL); captured launches hold the context's
+ * status word for that.
+ * `ws`: at least lssm_token_logprobs_workspace bytes of device memory, 8-byte
+ * aligned (0 bytes, NULL: rows short enough to need none); calls that may overlap need
+ * one each.  vocab <= LSSM_LOGPROB_MAX_VOCAB, rows <= LSSM_LOGPROB_MAX_ROWS,
+ * top_k <= LSSM_LOGPROB_MAX_TOP and vocab.  No counterpart in the reference, whose
+ * sampler forms probabilities on the host (sampler.cpp). */
+#define LSSM_LOGPROB_MAX_VOCAB 2097152
+#define LSSM_LOGPROB_MAX_ROWS 16777215
+#define LSSM_LOGPROB_MAX_TOP 64
+uint64_t lssm_token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t top_k);
+int lssm_token_logprobs(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                        float* logprob, float* entropy, float* stats, int32_t* top_ids,
+                        float* top_logprobs, uint32_t rows, uint32_t vocab, uint32_t top_k,
+                        lssm_dtype act, void* ws, uint64_t ws_bytes);
+/* The gradient of sum_r g_logprob[r] logprob[r] + g_entropy[r] entropy[r] to the
+ * logits, from the same logits and tokens and what lssm_token_logprobs left in
+ * stats and entropy (entropy may be NULL without g_entropy; g_logprob,
+ * g_entropy NULL: zero):
+ *   d_logits[r, v] = g_logprob ([v = t] - p_v) - g_entropy p_v (log p_v + entropy)
+ * rounded once.  d_logits may be logits (equal strides). */
+int lssm_token_logprobs_bwd(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                            const float* stats, const float* entropy, const float* g_logprob,
+                            const float* g_entropy, void* d_logits, uint32_t d_stride, uint32_t rows,
+                            uint32_t vocab, lssm_dtype act);
+/* Both at once, where the upstream gradients do not hang on the log
+ * probabilities (a mean negative log likelihood): each logit is read once where
+ * a row fits one workgroup's registers.  entropy and stats are needed, logprob
+ * may be NULL; ws as for lssm_token_logprobs with top_k 0. */
+int lssm_token_logprobs_grad(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                             const float* g_logprob, const float* g_entropy, float* logprob,
+                             float* entropy, float* stats, void* d_logits, uint32_t d_stride,
+                             uint32_t rows, uint32_t vocab, lssm_dtype act, void* ws, uint64_t ws_bytes);
 
 /* ------------------------------------------------------------------------- */
 /* Engine: whole-model prefill / decode (configs 3-5)                         */

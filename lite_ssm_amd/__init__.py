@@ -164,6 +164,10 @@ _SIGS = {
     "lssm_mixer_decode": ([_vp] * 16 + [_u32] * 8 + [_f, _i, _i], _i),
     "lssm_embed": ([_vp, _vp, _vp, _vp, _u32, _u32, _u32, _i], _i),
     "lssm_argmax": ([_vp, _vp, _vp, _u32, _u32, _i], _i),
+    "lssm_token_logprobs_workspace": ([_u32, _u32, _u32], C.c_uint64),
+    "lssm_token_logprobs": ([_vp, _vp, _u32] + [_vp] * 6 + [_u32] * 3 + [_i, _vp, C.c_uint64], _i),
+    "lssm_token_logprobs_bwd": ([_vp, _vp, _u32] + [_vp] * 6 + [_u32] * 3 + [_i], _i),
+    "lssm_token_logprobs_grad": ([_vp, _vp, _u32] + [_vp] * 7 + [_u32] * 3 + [_i, _vp, C.c_uint64], _i),
     # engine
     "lssm_engine_create": ([C.POINTER(_vp), _vp, C.POINTER(ModelConfig), _vp, _vp, _vp,
                             C.POINTER(LayerWeights), _u32, _u32], _i),
@@ -231,6 +235,11 @@ def _p(x):
     return x.data_ptr()
 
 
+def _nbytes(x):
+    """Bytes of a workspace tensor (0 for None)."""
+    return 0 if x is None else x.numel() * x.element_size()
+
+
 class Ctx:
     """One lssm_ctx: a HIP stream plus the batch flag (MetalOps analogue).
 
@@ -294,3 +303,26 @@ class Ctx:
     def ssd_step(self, x, B, Cm, dt, dt_bias, A_log, D, state, y, batch, dims, act):
         check(lib.lssm_ssd_step(self.h, _p(x), _p(B), _p(Cm), _p(dt), _p(dt_bias), _p(A_log),
                                 _p(D), _p(state), _p(y), batch, dims, act))
+
+    # log probabilities: entry points' arguments in order, packed rows unless a
+    # stride is given; ws is a device tensor of the workspace's bytes, or None
+    def token_logprobs_workspace(self, rows, vocab, top_k=0) -> int:
+        return int(lib.lssm_token_logprobs_workspace(rows, vocab, top_k))
+
+    def token_logprobs(self, logits, tokens, logprob, entropy, stats, top_ids, top_logprobs, rows, vocab,
+                       top_k, act, ws=None, stride=0):
+        check(lib.lssm_token_logprobs(self.h, _p(logits), stride, _p(tokens), _p(logprob), _p(entropy),
+                                      _p(stats), _p(top_ids), _p(top_logprobs), rows, vocab, top_k, act,
+                                      _p(ws), _nbytes(ws)))
+
+    def token_logprobs_bwd(self, logits, tokens, stats, entropy, g_logprob, g_entropy, d_logits, rows, vocab,
+                           act, stride=0, d_stride=0):
+        check(lib.lssm_token_logprobs_bwd(self.h, _p(logits), stride, _p(tokens), _p(stats), _p(entropy),
+                                          _p(g_logprob), _p(g_entropy), _p(d_logits), d_stride, rows, vocab,
+                                          act))
+
+    def token_logprobs_grad(self, logits, tokens, g_logprob, g_entropy, logprob, entropy, stats, d_logits,
+                            rows, vocab, act, ws=None, stride=0, d_stride=0):
+        check(lib.lssm_token_logprobs_grad(self.h, _p(logits), stride, _p(tokens), _p(g_logprob),
+                                           _p(g_entropy), _p(logprob), _p(entropy), _p(stats), _p(d_logits),
+                                           d_stride, rows, vocab, act, _p(ws), _nbytes(ws)))

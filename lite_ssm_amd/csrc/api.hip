@@ -556,6 +556,133 @@ int lssm_argmax(lssm_ctx* ctx, const void* logits, int32_t* ids, uint32_t rows, 
 }
 
 // ---------------------------------------------------------------------------
+// Log probabilities
+// ---------------------------------------------------------------------------
+namespace {
+
+int logprob_checks(const LogprobArgs& a, int act, const char* name) {
+    const size_t es = dtype_size(act);
+    LSSM_REQUIRE(a.V >= 1 && a.V <= LSSM_LOGPROB_MAX_VOCAB, "%s: vocab must be in [1, %d]", name, LSSM_LOGPROB_MAX_VOCAB);
+    LSSM_REQUIRE(a.rows <= LSSM_LOGPROB_MAX_ROWS, "%s: rows must be <= %d", name, LSSM_LOGPROB_MAX_ROWS);
+    LSSM_REQUIRE(a.x, "%s: null logits", name);
+    LSSM_REQUIRE(a.stride >= a.V && (!a.dx || a.dx_stride >= a.V), "%s: row stride smaller than the row", name);
+    LSSM_REQUIRE((uintptr_t)a.x % es == 0 && (uintptr_t)a.dx % es == 0, "%s: logits not aligned to their type", name);
+    for (const void* p : {(const void*)a.tokens, (const void*)a.logprob, (const void*)a.entropy, (const void*)a.stats,
+                          (const void*)a.top_ids, (const void*)a.top_logprobs, (const void*)a.g_logprob,
+                          (const void*)a.g_entropy})
+        LSSM_REQUIRE((uintptr_t)p % 4 == 0, "%s: arrays must be 4-byte aligned", name);
+    LSSM_REQUIRE(a.tokens || (!a.logprob && !a.g_logprob), "%s: log probabilities need tokens", name);
+    return LSSM_OK;
+}
+
+int logprob_ws_check(const LogprobArgs& a, int act, const void* ws, uint64_t ws_bytes, const char* name) {
+    if (logprob_segments(a.rows, a.V, act) == 1) return LSSM_OK;
+    const size_t need = logprob_ws_bytes(a.rows, a.V, a.K);
+    LSSM_REQUIRE(ws && ws_bytes >= need, "%s: the workspace needs %zu bytes", name, need);
+    LSSM_REQUIRE((uintptr_t)ws % 8 == 0, "%s: the workspace must be 8-byte aligned", name);
+    return LSSM_OK;
+}
+
+}  // namespace
+
+uint64_t lssm_token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t top_k) {
+    if (vocab > LSSM_LOGPROB_MAX_VOCAB || rows > LSSM_LOGPROB_MAX_ROWS || top_k > LSSM_LOGPROB_MAX_TOP) return 0;
+    return logprob_ws_bytes(rows, vocab, top_k);
+}
+
+int lssm_token_logprobs(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                        float* logprob, float* entropy, float* stats, int32_t* top_ids,
+                        float* top_logprobs, uint32_t rows, uint32_t vocab, uint32_t top_k,
+                        lssm_dtype act, void* ws, uint64_t ws_bytes) {
+    LSSM_CHECK_CTX(ctx);
+    const char* name = "token_logprobs";
+    LSSM_REQUIRE(valid_act(act), "%s: unknown dtype", name);
+    if (rows == 0) return LSSM_OK;
+    LogprobArgs a{};
+    a.x = logits;
+    a.stride = stride ? stride : vocab;
+    a.tokens = tokens;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.stats = stats;
+    a.top_ids = top_ids;
+    a.top_logprobs = top_logprobs;
+    a.rows = rows;
+    a.V = vocab;
+    a.K = top_k;
+    a.status = ctx->status;
+    if (int rc = logprob_checks(a, act, name)) return rc;
+    LSSM_REQUIRE(top_k <= LSSM_LOGPROB_MAX_TOP && top_k <= vocab, "%s: top_k must be <= vocab and %d", name,
+                 LSSM_LOGPROB_MAX_TOP);
+    LSSM_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "%s: top_k without top_ids and top_logprobs", name);
+    if (int rc = logprob_ws_check(a, act, ws, ws_bytes, name)) return rc;
+    hipError_t e = launch_logprobs(ctx->stream, a, act, ws);
+    if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
+    return finish(ctx, name);
+}
+
+int lssm_token_logprobs_bwd(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                            const float* stats, const float* entropy, const float* g_logprob,
+                            const float* g_entropy, void* d_logits, uint32_t d_stride, uint32_t rows,
+                            uint32_t vocab, lssm_dtype act) {
+    LSSM_CHECK_CTX(ctx);
+    const char* name = "token_logprobs_bwd";
+    LSSM_REQUIRE(valid_act(act), "%s: unknown dtype", name);
+    if (rows == 0) return LSSM_OK;
+    LogprobArgs a{};
+    a.x = logits;
+    a.stride = stride ? stride : vocab;
+    a.tokens = tokens;
+    a.entropy = const_cast<float*>(entropy);
+    a.stats = const_cast<float*>(stats);
+    a.g_logprob = g_logprob;
+    a.g_entropy = g_entropy;
+    a.dx = d_logits;
+    a.dx_stride = d_stride ? d_stride : vocab;
+    a.rows = rows;
+    a.V = vocab;
+    a.status = ctx->status;
+    if (int rc = logprob_checks(a, act, name)) return rc;
+    LSSM_REQUIRE(d_logits && stats, "%s: null d_logits or stats", name);
+    LSSM_REQUIRE(!g_entropy || entropy, "%s: g_entropy needs the entropies", name);
+    LSSM_REQUIRE(d_logits != logits || a.stride == a.dx_stride, "%s: in place needs equal strides", name);
+    hipError_t e = launch_logprobs_grad(ctx->stream, a, act);
+    if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
+    return finish(ctx, name);
+}
+
+int lssm_token_logprobs_grad(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
+                             const float* g_logprob, const float* g_entropy, float* logprob,
+                             float* entropy, float* stats, void* d_logits, uint32_t d_stride,
+                             uint32_t rows, uint32_t vocab, lssm_dtype act, void* ws, uint64_t ws_bytes) {
+    LSSM_CHECK_CTX(ctx);
+    const char* name = "token_logprobs_grad";
+    LSSM_REQUIRE(valid_act(act), "%s: unknown dtype", name);
+    if (rows == 0) return LSSM_OK;
+    LogprobArgs a{};
+    a.x = logits;
+    a.stride = stride ? stride : vocab;
+    a.tokens = tokens;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.stats = stats;
+    a.g_logprob = g_logprob;
+    a.g_entropy = g_entropy;
+    a.dx = d_logits;
+    a.dx_stride = d_stride ? d_stride : vocab;
+    a.rows = rows;
+    a.V = vocab;
+    a.status = ctx->status;
+    if (int rc = logprob_checks(a, act, name)) return rc;
+    LSSM_REQUIRE(d_logits && stats && entropy, "%s: null d_logits, stats or entropy", name);
+    LSSM_REQUIRE(d_logits != logits || a.stride == a.dx_stride, "%s: in place needs equal strides", name);
+    if (int rc = logprob_ws_check(a, act, ws, ws_bytes, name)) return rc;
+    hipError_t e = launch_logprobs(ctx->stream, a, act, ws);
+    if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
+    return finish(ctx, name);
+}
+
+// ---------------------------------------------------------------------------
 // Reference-named entries (fp16, batch 1)
 // ---------------------------------------------------------------------------
 int lssm_rmsnorm_f16(lssm_ctx* ctx, const void* x, const void* w, void* y, lssm_rmsnorm_dims d) {

@@ -54,6 +54,10 @@ int sync_and_check(lssm_ctx* ctx, const char* what) {
                          wait_msg);
     if (st & STATUS_BAD_TOKEN)
         return set_error(LSSM_EINVAL, "Mamba2Model::embed: token_id out of range (%s)", what);
+    if (st & STATUS_BAD_TARGET)
+        return set_error((st & STATUS_WAIT_TIMEOUT) ? LSSM_EDEVICE : LSSM_EINVAL,
+                         "token_logprobs: a token is not below the vocabulary (%s)%s%s", what,
+                         (st & STATUS_WAIT_TIMEOUT) ? "; also: " : "", (st & STATUS_WAIT_TIMEOUT) ? wait_msg : "");
     return set_error(LSSM_EDEVICE, "%s: %s", what, wait_msg);
 }
 
@@ -223,6 +227,8 @@ static const char* const kKernelNames[] = {
     "inproj_decode",
     "embed",
     "argmax",
+    "token_logprobs",
+    "token_logprobs_bwd",
 };
 
 int lssm_kernel_count(void) { return (int)(sizeof(kKernelNames) / sizeof(kKernelNames[0])); }

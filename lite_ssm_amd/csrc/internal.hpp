@@ -59,6 +59,7 @@ void clear_error();
 // Bits of lssm_ctx::status.
 constexpr uint32_t STATUS_BAD_TOKEN = 1u;      // a token id outside [0, vocab) reached the embedding
 constexpr uint32_t STATUS_WAIT_TIMEOUT = 2u;   // a cross-workgroup wait gave up (not co-resident)
+constexpr uint32_t STATUS_BAD_TARGET = 4u;     // a token to score is not below the vocabulary
 
 // After enqueueing an op: report launch errors; outside a batch, also wait and
 // report asynchronous kernel failures and the device status word.
@@ -132,6 +133,36 @@ hipError_t launch_argmax(hipStream_t s, const void* logits, int32_t* ids, uint32
 // ids[0] = the first index of the maximum over *nblk partials (pv, pi)
 hipError_t launch_argmax_final(hipStream_t s, const float* pv, const int* pi, const uint32_t* nblk,
                                int32_t* ids);
+
+// Log probabilities (logprobs.hip): rows of V logits, row strides in elements.
+// tokens / logprob / entropy / stats / g_logprob / g_entropy may be null; K
+// alternatives a row.  dx: the gradient too.  A row is cut into
+// logprob_segments segments; more than one needs a workspace.
+struct LogprobArgs {
+    const void* x;
+    size_t stride;
+    const int32_t* tokens;
+    float* logprob;
+    float* entropy;
+    float* stats;
+    int32_t* top_ids;
+    float* top_logprobs;
+    const float* g_logprob;
+    const float* g_entropy;
+    void* dx;
+    size_t dx_stride;
+    uint32_t rows, V, K;
+    uint32_t* status;
+    // set by the launchers
+    uint32_t S, seg_vecs;
+    float* part;
+    unsigned long long* part_keys;
+};
+size_t logprob_ws_bytes(uint32_t rows, uint32_t vocab, uint32_t top_k);
+uint32_t logprob_segments(uint32_t rows, uint32_t vocab, int act);
+hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws);
+// the gradient alone, from kept statistics
+hipError_t launch_logprobs_grad(hipStream_t s, LogprobArgs a, int act);
 
 // appends next[0..B) as row *pos of log [cap][B] and advances *pos (B <= 64)
 hipError_t launch_id_log(hipStream_t s, const int32_t* next, uint32_t B, int32_t* log, uint32_t cap,

@@ -1,0 +1,526 @@
+// logprobs.hip — log probabilities of given tokens under rows of logits, their
+// entropies and best alternatives, and the gradient to the logits.
+//
+// A row x of V logits and a token t:
+//   m = max x,  S = sum e^{x - m},  ls = log S,  T = sum e^{x - m} (x - m)
+//   log p(v) = (x_v - m) - ls,  H = -sum p log p = ls - T / S
+//   d log p(t) / dx_v = [v = t] - p_v,  dH / dx_v = -p_v (log p_v + H)
+// (max, ls) are kept instead of log-sum-exp: their sum would lose up to
+// 2^-24 |m| where the two numbers do not.
+//
+// A block reads one segment of a row into registers, once: all of its loads
+// are in flight together, and the maximum, the sums, the alternatives and the
+// gradient are passes over registers.  A row of more than LP_MAXV vectors, or
+// one of few rows, is cut into segments that a second launch joins.
+//
+// Masked logits: -inf has p = 0 and adds nothing (p log p is 0 there);
+// the type's lowest value is an ordinary number.  A row with nothing but -inf
+// has log p = -inf, H = 0, statistics (0, inf) and a zero gradient.  A NaN or
+// +inf makes its row NaN.
+#include <algorithm>
+#include <cfloat>
+#include <cstdint>
+#include <type_traits>
+
+#include "common.hpp"
+#include "internal.hpp"
+
+namespace lssm {
+
+namespace {
+
+constexpr int LP_NT = 1024;                  // threads of a segment's block
+constexpr int LP_NW = LP_NT / WAVE;
+constexpr int LP_MAXR = 8;                   // 16-byte vectors a thread holds
+constexpr int LP_CAP = 1024;                 // candidates of a segment's alternatives
+constexpr int LP_TAIL = LP_NT / 2;           // first thread of those that take a row's ragged end
+constexpr float LOG2E = 1.44269504088896341f;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
+
+__device__ __forceinline__ float mul0(float a, float b) { return a == 0.0f ? 0.0f : a * b; }
+__device__ __forceinline__ float exp_fast(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+// An exponent as a factor of its own e^d: below -200 e^d is 0, and so is the
+// product, also for -inf.  (A NaN is lost here; e^d keeps it.)
+__device__ __forceinline__ float factor(float d) { return fmaxf(d, -200.0f); }
+
+template <typename T> struct Vec { static constexpr int E = 16 / sizeof(T); };
+
+// element e (compile-time after unrolling) of a 16-byte vector
+template <typename T> __device__ __forceinline__ float elem(const u32x4& q, int e) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(q[e]);
+    } else {
+        const uint32_t w = q[e / 2];
+        if constexpr (__is_same(T, bf16)) return __uint_as_float((e & 1) ? (w & 0xffff0000u) : (w << 16));
+        else return f_of_bits<T>((uint16_t)((e & 1) ? (w >> 16) : w));
+    }
+}
+template <typename T> __device__ __forceinline__ uint32_t neg_inf_word() {
+    return sizeof(T) == 4 ? 0xff800000u : (__is_same(T, bf16) ? 0xff80ff80u : 0xfc00fc00u);
+}
+
+// Order of the alternatives: larger value first, then the lower index.  0: no
+// alternative (-inf, NaN).  -0 and +0 are equal.
+__device__ __forceinline__ uint32_t ord_of(float v) {
+    if (!(v > -INFINITY)) return 0u;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float of_ord(uint32_t o) {
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ u64 key_of(uint32_t ord, uint32_t idx) { return ((u64)ord << 32) | (uint32_t)~idx; }
+
+// Maximum over the wave, in every lane.
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    v = fmaxf(v, dpp_f32<0x141>(v));
+    v = fmaxf(v, dpp_f32<0x140>(v));
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+// (m, S, T) of a set of logits relative to its maximum m; moved to a larger
+// reference M.  An empty set is (-FLT_MAX, 0, 0).
+struct Soft { float m, S, T; };
+__device__ __forceinline__ Soft moved(Soft a, float M) {
+    const float d = a.m - M, f = d == 0.0f ? 1.0f : exp_fast(d);
+    return {M, a.S * f, mul0(f, a.T + mul0(a.S, d))};
+}
+
+// Keeps a pass over the registers from leaving its unpacked values to the next
+// (16-bit logits: twice the registers, and spills).
+template <int R> __device__ __forceinline__ void repack(u32x4 (&q)[R]) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) asm volatile("" : "+v"(q[i]));
+}
+
+// What a row gives in the end.
+struct RowOut { float max, ls, H; };
+__device__ __forceinline__ RowOut row_out(Soft a) {
+    if (a.S == 0.0f) return {0.0f, INFINITY, 0.0f};     // nothing left
+    const float ls = logf(a.S);
+    return {a.m < INFINITY ? a.m + 0.0f * ls : a.m, ls, ls - a.T / a.S};     // (a NaN shows in the maximum too)
+}
+
+__device__ __forceinline__ void store_row(const LogprobArgs& a, uint32_t r, const RowOut& o, float xt, int t) {
+    if (a.logprob) a.logprob[r] = t < 0 ? 0.0f : ((uint32_t)t < a.V ? (xt - o.max) - o.ls : NAN);
+    if (a.entropy) a.entropy[r] = o.H;
+    if (a.stats) {
+        a.stats[2 * (size_t)r] = o.max;
+        a.stats[2 * (size_t)r + 1] = o.ls;
+    }
+    if (t >= 0 && (uint32_t)t >= a.V) atomicOr(a.status, STATUS_BAD_TARGET);
+}
+
+// The K best of n unique keys in LDS: the rank of a key is the number of
+// larger ones, so the order in which they were collected does not show.
+template <int NT, typename F> __device__ __forceinline__ void rank_keys(const u64* keys, uint32_t n, uint32_t K, F put) {
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
+        const u64 k = keys[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += keys[j] > k ? 1u : 0u;
+        if (rank < K) put(rank, k);
+    }
+}
+
+// Gradient of one logit; p = 0 where it is masked, whatever log p is.
+__device__ __forceinline__ float grad_of(float x, float max, float ls, float H, float g, float ge) {
+    const float lp = (x - max) - ls, p = exp_fast(lp);
+    return -p * fmaf(ge, factor(lp) + H, g);
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(a)) |
+           ((uint32_t)__builtin_bit_cast(uint16_t, from_f<T>(b)) << 16);
+}
+
+// Where a row's 16-byte vectors lie: `head` elements before the first aligned
+// address, then nv vectors, the rest behind them.
+template <typename T> struct RowSpan {
+    uint32_t head, nv, tail0;
+    __device__ RowSpan(const T* row, uint32_t V) {
+        head = min(V, (uint32_t)(((16u - ((uintptr_t)row & 15u)) & 15u) / sizeof(T)));
+        nv = (V - head) / Vec<T>::E;
+        tail0 = head + nv * Vec<T>::E;
+    }
+};
+
+// One segment of a row (the whole row where a.S == 1).
+// GRAD (a.S == 1, no alternatives): the gradient is written from the registers too.
+template <typename T, int R, bool GRAD>
+__global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
+    constexpr int E = Vec<T>::E;
+    __shared__ float sm[LP_NW], sS[LP_NW], sT[LP_NW];
+    __shared__ uint32_t stau[LP_NW], scount;
+    __shared__ u64 keys[LP_CAP];
+    __shared__ u64 swin[LP_NW];
+    const uint32_t r = blockIdx.x / a.S, seg = blockIdx.x % a.S;
+    const uint32_t tid = threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const T* row = (const T*)a.x + (size_t)r * a.stride;
+    const RowSpan<T> sp(row, a.V);
+    const uint32_t v0 = seg * a.seg_vecs, v1 = min(sp.nv, v0 + a.seg_vecs);
+    const u32x4* vecs = reinterpret_cast<const u32x4*>(row + sp.head);
+
+    u32x4 q[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const uint32_t v = v0 + i * LP_NT + tid;
+        const uint32_t n = neg_inf_word<T>();
+        q[i] = v < v1 ? vecs[v] : u32x4{n, n, n, n};
+    }
+    // the ragged ends: threads 0.. those before the first vector (first
+    // segment), threads LP_TAIL.. those behind the last (last segment)
+    float xe = -INFINITY;
+    uint32_t ie = a.V;
+    if (seg == 0 && tid < sp.head) ie = tid;
+    if (seg + 1 == a.S && tid >= LP_TAIL && sp.tail0 + (tid - LP_TAIL) < a.V) ie = sp.tail0 + (tid - LP_TAIL);
+    if (ie < a.V) xe = to_f(row[ie]);
+
+    // the given token's logit, read before any gradient may replace it
+    int t = -1;
+    float xt = 0.0f;
+    if ((GRAD || tid == 0) && a.S == 1 && a.tokens) {
+        t = a.tokens[r];
+        if (tid == 0 && t >= 0 && (uint32_t)t < a.V) xt = to_f(row[t]);
+    }
+
+    float m = fmaxf(-FLT_MAX, xe);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, elem<T>(q[i], e));
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    repack(q);
+    float S, U;
+    {
+        const float d = xe - m;
+        S = exp_fast(d);
+        U = S * factor(d);
+    }
+    float S2 = 0.0f, U2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = elem<T>(q[i], e) - m, x = exp_fast(d);
+            (e & 1 ? S2 : S) += x;
+            (e & 1 ? U2 : U) = fmaf(x, factor(d), e & 1 ? U2 : U);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    S += S2;
+    U += U2;
+    const float mw = wave_max(m);
+    Soft s = moved({m, S, U}, mw);
+    s.S = wave_sum(s.S);
+    s.T = wave_sum(s.T);
+    const uint32_t K = GRAD ? 0u : a.K;
+    if (tid % WAVE == 0) {
+        sm[w] = mw;
+        sS[w] = s.S;
+        sT[w] = s.T;
+    }
+    if (K) {
+        // the K-th best of the lanes' best values: at least K of the wave's
+        // values are no less, or tau is no more than the lowest finite one
+        // (which stands for lanes without a value).  Found bit by bit.
+        const uint32_t best = ord_of(m);
+        uint32_t tau = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t c = tau | (1u << bit);
+            if ((uint32_t)__popcll(__ballot(best >= c)) >= K) tau = c;
+        }
+        if (tid % WAVE == 0) stau[w] = tau;
+        if (tid == 0) scount = 0;
+    }
+    __syncthreads();
+    // all waves' sums (lanes 16 and up repeat the first 16)
+    const int l = tid % LP_NW;
+    const float M = wave_max(sm[l]);
+    Soft b = moved({sm[l], sS[l], sT[l]}, M);
+    b.S = group_sum<LP_NW>(b.S);
+    b.T = group_sum<LP_NW>(b.T);
+    const RowOut o = row_out(b);
+    if (tid == 0) {
+        if (a.S == 1) {
+            store_row(a, r, o, xt, t);
+        } else {
+            float* p = a.part + 3 * (size_t)blockIdx.x;
+            p[0] = b.m;
+            p[1] = b.S;
+            p[2] = b.T;
+        }
+    }
+    if (K) {
+        uint32_t tau = 1;
+        for (int i = 0; i < LP_NW; ++i) tau = max(tau, stau[i]);
+        auto each = [&](auto f) {
+            repack(q);
+            uint32_t vb = v0 + tid;
+            asm volatile("" : "+v"(vb));       // nor its places
+            if (ie < a.V) f(ord_of(xe), ie);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const uint32_t v = vb + i * LP_NT;
+                if (v < v1) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) f(ord_of(elem<T>(q[i], e)), sp.head + v * E + e);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        if (ord_of(m) >= tau)
+            each([&](uint32_t ov, uint32_t idx) {
+                if (ov >= tau) {
+                    const uint32_t at = atomicAdd(&scount, 1u);
+                    if (at < LP_CAP) keys[at] = key_of(ov, idx);
+                }
+            });
+        __syncthreads();
+        const uint32_t n = scount;
+        auto put = [&](uint32_t rank, u64 k) {
+            const uint32_t idx = ~(uint32_t)k;
+            if (a.S == 1) {
+                const float v = of_ord((uint32_t)(k >> 32));
+                a.top_ids[(size_t)r * K + rank] = k ? (int)idx : -1;
+                a.top_logprobs[(size_t)r * K + rank] = k ? (v - o.max) - o.ls : -INFINITY;
+            } else {
+                a.part_keys[(size_t)blockIdx.x * K + rank] = k;
+            }
+        };
+        if (n <= LP_CAP) {
+            rank_keys<LP_NT>(keys, n, K, put);
+            for (uint32_t i = n + tid; i < K; i += LP_NT) put(i, 0);
+        } else {
+            // more equal (or masked) values than the list holds: one after the
+            // other, the best key below the last
+            u64 last = ~0ull;
+            for (uint32_t i = 0; i < K; ++i) {
+                u64 k = 0;
+                each([&](uint32_t ov, uint32_t idx) {
+                    const u64 c = ov ? key_of(ov, idx) : 0;
+                    if (c < last && c > k) k = c;
+                });
+#pragma unroll
+                for (int sft = 1; sft < WAVE; sft <<= 1) {
+                    const u64 c = __shfl_xor(k, sft);
+                    k = c > k ? c : k;
+                }
+                if (tid % WAVE == 0) swin[w] = k;
+                __syncthreads();
+                k = 0;
+                for (int j = 0; j < LP_NW; ++j) k = swin[j] > k ? swin[j] : k;
+                __syncthreads();
+                if (tid == 0) put(i, k);
+                last = k;
+            }
+        }
+    }
+    if constexpr (GRAD) {
+        const float g = (a.g_logprob && t >= 0 && (uint32_t)t < a.V) ? a.g_logprob[r] : 0.0f;
+        const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
+        const float hot = o.ls == INFINITY ? 0.0f : g;
+        T* dx = (T*)a.dx + (size_t)r * a.dx_stride;
+        const bool vec = (((uintptr_t)dx - (uintptr_t)row) & 15u) == 0;
+        repack(q);
+        if (ie < a.V) dx[ie] = from_f<T>(grad_of(xe, o.max, o.ls, o.H, g, ge) + ((int)ie == t ? hot : 0.0f));
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const uint32_t v = v0 + i * LP_NT + tid;
+            if (v < v1) {
+                const uint32_t idx = sp.head + v * E;
+                float d[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) d[e] = grad_of(elem<T>(q[i], e), o.max, o.ls, o.H, g, ge);
+                if ((uint32_t)t - idx < (uint32_t)E) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (idx + e == (uint32_t)t) d[e] += hot;
+                }
+                if (vec) {
+                    u32x4 s4;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (sizeof(T) == 4) s4[k] = __float_as_uint(d[k]);
+                        else s4[k] = pack2<T>(d[2 * k], d[2 * k + 1]);
+                    }
+                    *reinterpret_cast<u32x4*>(dx + idx) = s4;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) dx[idx + e] = from_f<T>(d[e]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
+// Joins a row's segments: the sums, then the best of the segments' best.
+template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a) {
+    extern __shared__ u64 jkeys[];
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, S = a.S, K = a.K;
+    const float* p = a.part + 3 * (size_t)r * S;
+    Soft s{-FLT_MAX, 0.0f, 0.0f};
+    for (uint32_t i = tid % WAVE; i < S; i += WAVE) {
+        const Soft n{p[3 * i], p[3 * i + 1], p[3 * i + 2]};
+        const float M = fmaxf(s.m, n.m);
+        const Soft x = moved(s, M), y = moved(n, M);
+        s = {M, x.S + y.S, x.T + y.T};
+    }
+    s = moved(s, wave_max(s.m));
+    s.S = wave_sum(s.S);
+    s.T = wave_sum(s.T);
+    const RowOut o = row_out(s);
+    if (tid == 0) {
+        const int t = a.tokens ? a.tokens[r] : -1;
+        const T* row = (const T*)a.x + (size_t)r * a.stride;
+        store_row(a, r, o, t >= 0 && (uint32_t)t < a.V ? to_f(row[t]) : 0.0f, t);
+    }
+    if (K == 0) return;
+    const uint32_t n = S * K;
+    for (uint32_t i = tid; i < n; i += 256) jkeys[i] = a.part_keys[(size_t)r * n + i];
+    __syncthreads();
+    __shared__ uint32_t found;
+    if (tid == 0) found = 0;
+    __syncthreads();
+    rank_keys<256>(jkeys, n, K, [&](uint32_t rank, u64 k) {
+        if (!k) return;                        // an empty place
+        atomicAdd(&found, 1u);
+        a.top_ids[(size_t)r * K + rank] = (int)~(uint32_t)k;
+        a.top_logprobs[(size_t)r * K + rank] = (of_ord((uint32_t)(k >> 32)) - o.max) - o.ls;
+    });
+    __syncthreads();
+    for (uint32_t i = found + tid; i < K; i += 256) {
+        a.top_ids[(size_t)r * K + i] = -1;
+        a.top_logprobs[(size_t)r * K + i] = -INFINITY;
+    }
+}
+
+// The gradient from kept statistics: one pass, a block a stretch of a row.
+constexpr int LG_NT = 256, LG_R = 4;
+template <typename T> __global__ __launch_bounds__(LG_NT) void logprob_grad_kernel(LogprobArgs a) {
+    constexpr int E = Vec<T>::E;
+    const uint32_t r = blockIdx.x / a.S, seg = blockIdx.x % a.S, tid = threadIdx.x;
+    const T* row = (const T*)a.x + (size_t)r * a.stride;
+    T* dx = (T*)a.dx + (size_t)r * a.dx_stride;
+    const RowSpan<T> sp(row, a.V);
+    const u32x4* vecs = reinterpret_cast<const u32x4*>(row + sp.head);
+    const uint32_t v0 = seg * (LG_NT * LG_R);
+    u32x4 q[LG_R];
+#pragma unroll
+    for (int i = 0; i < LG_R; ++i) {
+        const uint32_t v = v0 + i * LG_NT + tid;
+        q[i] = v < sp.nv ? vecs[v] : u32x4{0, 0, 0, 0};
+    }
+    const float mx = a.stats[2 * (size_t)r], ls = a.stats[2 * (size_t)r + 1];
+    const float H = a.entropy ? a.entropy[r] : 0.0f;
+    const int t = a.tokens ? a.tokens[r] : -1;
+    const float g = (a.g_logprob && t >= 0 && (uint32_t)t < a.V) ? a.g_logprob[r] : 0.0f;
+    const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
+    const float hot = ls == INFINITY ? 0.0f : g;
+    if (seg == 0 && tid == 0 && t >= 0 && (uint32_t)t >= a.V) atomicOr(a.status, STATUS_BAD_TARGET);
+    const bool vec = (((uintptr_t)dx - (uintptr_t)row) & 15u) == 0;
+    uint32_t ie = a.V;
+    if (seg == 0 && tid < sp.head) ie = tid;
+    if (seg == 0 && tid >= LG_NT / 2 && sp.tail0 + (tid - LG_NT / 2) < a.V) ie = sp.tail0 + (tid - LG_NT / 2);
+    if (ie < a.V) dx[ie] = from_f<T>(grad_of(to_f(row[ie]), mx, ls, H, g, ge) + ((int)ie == t ? hot : 0.0f));
+#pragma unroll
+    for (int i = 0; i < LG_R; ++i) {
+        const uint32_t v = v0 + i * LG_NT + tid;
+        if (v >= sp.nv) continue;
+        const uint32_t idx = sp.head + v * E;
+        float d[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) d[e] = grad_of(elem<T>(q[i], e), mx, ls, H, g, ge);
+        if ((uint32_t)t - idx < (uint32_t)E) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (idx + e == (uint32_t)t) d[e] += hot;
+        }
+        if (vec) {
+            u32x4 s4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if constexpr (sizeof(T) == 4) s4[k] = __float_as_uint(d[k]);
+                else s4[k] = pack2<T>(d[2 * k], d[2 * k + 1]);
+            }
+            *reinterpret_cast<u32x4*>(dx + idx) = s4;
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) dx[idx + e] = from_f<T>(d[e]);
+        }
+    }
+}
+
+template <typename F> hipError_t with_type(int act, F f) {
+    if (act == LSSM_BF16) return f(bf16{});
+    if (act == LSSM_F16) return f(f16{});
+    return f(float{});
+}
+
+}  // namespace
+
+// Segments of a row.
+uint32_t logprob_segments(uint32_t rows, uint32_t vocab, int act) {
+    (void)rows;
+    const uint32_t e = act == LSSM_F32 ? 4u : 8u;
+    return std::max(1u, (vocab / e + LP_NT * LP_MAXR - 1) / (LP_NT * LP_MAXR));
+}
+
+// [part: 3 floats a segment, to a multiple of 8 bytes][keys: K a segment]
+static size_t part_bytes(uint32_t rows, uint32_t segs) { return ((size_t)rows * segs * 12 + 7) / 8 * 8; }
+
+size_t logprob_ws_bytes(uint32_t rows, uint32_t vocab, uint32_t top_k) {
+    size_t n = 0;     // of either type size
+    for (int act : {LSSM_BF16, LSSM_F32}) {
+        const uint32_t S = logprob_segments(rows, vocab, act);
+        if (S > 1) n = std::max(n, part_bytes(rows, S) + (size_t)rows * S * top_k * 8);
+    }
+    return n;
+}
+
+hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws) {
+    a.S = logprob_segments(a.rows, a.V, act);
+    const uint32_t nv = a.V / (act == LSSM_F32 ? 4u : 8u);
+    a.seg_vecs = std::max(1u, (nv + a.S - 1) / a.S);
+    if (a.S > 1) {
+        a.part = static_cast<float*>(ws);
+        a.part_keys = reinterpret_cast<unsigned long long*>(static_cast<char*>(ws) + part_bytes(a.rows, a.S));
+    }
+    return with_type(act, [&](auto z) {
+        using T = decltype(z);
+        const dim3 grid(a.rows * a.S);
+        const bool grad = a.dx && a.S == 1;
+        auto go = [&](auto rc) {
+            constexpr int R = decltype(rc)::value;
+            if (grad) logprob_seg_kernel<T, R, true><<<grid, LP_NT, 0, s>>>(a);
+            else logprob_seg_kernel<T, R, false><<<grid, LP_NT, 0, s>>>(a);
+        };
+        if (a.seg_vecs <= 2 * LP_NT) go(std::integral_constant<int, 2>{});
+        else if (a.seg_vecs <= 4 * LP_NT) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 8>{});
+        if (a.S > 1) logprob_join_kernel<T><<<a.rows, 256, (size_t)a.S * a.K * 8, s>>>(a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || !a.dx || grad) return e;
+        return launch_logprobs_grad(s, a, act);
+    });
+}
+
+hipError_t launch_logprobs_grad(hipStream_t s, LogprobArgs a, int act) {
+    const uint32_t nv = a.V / (act == LSSM_F32 ? 4u : 8u);
+    a.S = std::max(1u, (nv + LG_NT * LG_R - 1) / (LG_NT * LG_R));
+    return with_type(act, [&](auto z) {
+        logprob_grad_kernel<decltype(z)><<<a.rows * a.S, LG_NT, 0, s>>>(a);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace lssm
