@@ -295,6 +295,28 @@ int lssm_ssd_chunked(lssm_ctx* ctx, const void* X, const void* B, const void* C,
                      const void* dt_raw, const void* dt_bias, const void* A_log,
                      const void* D_skip, void* Y, float* state, uint32_t batch,
                      lssm_ssd_dims dims, lssm_dtype act);
+/* The gradients of lssm_ssd_chunked, from the same inputs.  `state` is the state
+ * that entered the scan (lssm_ssd_chunked overwrites it: keep a copy; NULL =
+ * zeros), dY [batch, L, H, P] and d_state [batch, H, P, N] (fp32, NULL = zeros) the
+ * gradients of its outputs.  Writes dX, dB, dC, d_dt (of dt_raw), d_dt_bias, dA_log,
+ * dD (has_D) in the shapes and type of what they belong to, each rounded once, and
+ * d_state0 (fp32, or NULL), the gradient of `state`.  The scan is taken as exact
+ * (the forward's roundings have no gradient); dt outside [dt_min, dt_max] has none
+ * either.  dB and dC are summed over the heads of a group.  Sums, decays and states
+ * are held in fp32 or more, and every order of summation is fixed: the same inputs
+ * give the same bits.  dims.chunk_size does not matter here.  Outputs may not overlap inputs.
+ * `ws`: at least lssm_ssd_chunked_bwd_workspace bytes of device memory, 16-byte
+ * aligned (for refused dims the size is 0); calls that may overlap need one
+ * each.  P <= 1024, N <= 256, L <= LSSM_SSD_BWD_MAX_L.  No counterpart in the
+ * reference, which only runs trained models. */
+#define LSSM_SSD_BWD_MAX_L 1048576
+uint64_t lssm_ssd_chunked_bwd_workspace(uint32_t batch, lssm_ssd_dims dims, lssm_dtype act);
+int lssm_ssd_chunked_bwd(lssm_ctx* ctx, const void* X, const void* B, const void* C,
+                         const void* dt_raw, const void* dt_bias, const void* A_log,
+                         const void* D_skip, const float* state, const void* dY,
+                         const float* d_state, void* dX, void* dB, void* dC, void* d_dt,
+                         void* d_dt_bias, void* dA_log, void* dD, float* d_state0, uint32_t batch,
+                         lssm_ssd_dims dims, lssm_dtype act, void* ws, uint64_t ws_bytes);
 /* One decode step for `batch` sequences: x [batch, H, P], B/C [batch, G, N],
  * dt_raw [batch, H], state [batch, H, P, N] fp32 updated in place. */
 int lssm_ssd_step(lssm_ctx* ctx, const void* x, const void* B, const void* C,

@@ -157,6 +157,8 @@ _SIGS = {
     "lssm_gated_rmsnorm": ([_vp, _vp, _vp, _vp, _vp, _u32, _u32, _f, _i], _i),
     "lssm_norm_linear_decode": ([_vp, _vp, _vp, _f, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _i, _i, _i], _i),
     "lssm_ssd_chunked": ([_vp] + [_vp] * 9 + [_u32, SSDDims, _i], _i),
+    "lssm_ssd_chunked_bwd_workspace": ([_u32, SSDDims, _i], C.c_uint64),
+    "lssm_ssd_chunked_bwd": ([_vp] * 19 + [_u32, SSDDims, _i, _vp, C.c_uint64], _i),
     "lssm_ssd_step": ([_vp] + [_vp] * 9 + [_u32, SSDStepDims, _i], _i),
     "lssm_inproj_decode": ([_vp] * 11 + [_u32] * 7 + [_f, _i, _i], _i),
     "lssm_inproj_ssd_decode": ([_vp] * 14 + [_u32] * 8 + [_f, _i, _i], _i),
@@ -299,6 +301,16 @@ class Ctx:
     def ssd_chunked(self, X, B, Cm, dt, dt_bias, A_log, D, Y, state, batch, dims, act):
         check(lib.lssm_ssd_chunked(self.h, _p(X), _p(B), _p(Cm), _p(dt), _p(dt_bias), _p(A_log),
                                    _p(D), _p(Y), _p(state), batch, dims, act))
+
+    def ssd_chunked_bwd_workspace(self, batch, dims, act) -> int:
+        return int(lib.lssm_ssd_chunked_bwd_workspace(batch, dims, act))
+
+    def ssd_chunked_bwd(self, X, B, Cm, dt, dt_bias, A_log, D, state, dY, d_state, dX, dB, dC, d_dt, d_dt_bias,
+                        dA_log, dD, d_state0, batch, dims, act, ws):
+        check(lib.lssm_ssd_chunked_bwd(self.h, _p(X), _p(B), _p(Cm), _p(dt), _p(dt_bias), _p(A_log), _p(D),
+                                       _p(state), _p(dY), _p(d_state), _p(dX), _p(dB), _p(dC), _p(d_dt),
+                                       _p(d_dt_bias), _p(dA_log), _p(dD), _p(d_state0), batch, dims, act,
+                                       _p(ws), _nbytes(ws)))
 
     def ssd_step(self, x, B, Cm, dt, dt_bias, A_log, D, state, y, batch, dims, act):
         check(lib.lssm_ssd_step(self.h, _p(x), _p(B), _p(Cm), _p(dt), _p(dt_bias), _p(A_log),

@@ -314,6 +314,78 @@ int lssm_ssd_chunked(lssm_ctx* ctx, const void* X, const void* B, const void* C,
     return finish(ctx, "ssd_chunked");
 }
 
+namespace {
+
+int ssd_bwd_checks(uint32_t batch, const lssm_ssd_dims& d, lssm_dtype act, const char* name) {
+    LSSM_REQUIRE(valid_act(act), "%s: unknown dtype", name);
+    if (int rc = ssd_common_checks(d, name)) return rc;
+    LSSM_REQUIRE(batch <= 65535, "%s: batch must be <= 65535", name);
+    LSSM_REQUIRE(d.P <= 1024 && d.H <= 65535 && d.L <= LSSM_SSD_BWD_MAX_L, "%s: P must be <= 1024, H <= 65535, L <= %d", name,
+                 LSSM_SSD_BWD_MAX_L);
+    return LSSM_OK;
+}
+
+}  // namespace
+
+uint64_t lssm_ssd_chunked_bwd_workspace(uint32_t batch, lssm_ssd_dims d, lssm_dtype act) {
+    clear_error();
+    return ssd_bwd_checks(batch, d, act, "ssd_chunked_bwd") ? 0 : ssd_bwd_ws_bytes(batch, d, act);
+}
+
+int lssm_ssd_chunked_bwd(lssm_ctx* ctx, const void* X, const void* B, const void* C, const void* dt_raw,
+                         const void* dt_bias, const void* A_log, const void* D_skip, const float* state,
+                         const void* dY, const float* d_state, void* dX, void* dB, void* dC, void* d_dt,
+                         void* d_dt_bias, void* dA_log, void* dD, float* d_state0, uint32_t batch,
+                         lssm_ssd_dims d, lssm_dtype act, void* ws, uint64_t ws_bytes) {
+    LSSM_CHECK_CTX(ctx);
+    const char* name = "ssd_chunked_bwd";
+    if (int rc = ssd_bwd_checks(batch, d, act, name)) return rc;
+    LSSM_REQUIRE(!d.has_D || (D_skip && dD), "%s: has_D set but D or dD is null", name);
+    LSSM_REQUIRE(dt_bias && A_log && d_dt_bias && dA_log, "%s: null pointer", name);
+    LSSM_REQUIRE(batch == 0 || d.L == 0 || (X && B && C && dt_raw && dY && dX && dB && dC && d_dt),
+                 "%s: null pointer", name);
+    const size_t es = dtype_size(act);
+    for (const void* p : {X, B, C, dt_raw, dt_bias, A_log, D_skip, dY, (const void*)dX, (const void*)dB,
+                          (const void*)dC, (const void*)d_dt, (const void*)d_dt_bias, (const void*)dA_log,
+                          (const void*)dD})
+        LSSM_REQUIRE((uintptr_t)p % es == 0, "%s: arrays must be aligned to their type", name);
+    for (const void* p : {(const void*)state, (const void*)d_state, (const void*)d_state0})
+        LSSM_REQUIRE((uintptr_t)p % 4 == 0, "%s: states must be 4-byte aligned", name);
+    const size_t need = ssd_bwd_ws_bytes(batch, d, act);
+    LSSM_REQUIRE(need == 0 || (ws && ws_bytes >= need), "%s: the workspace needs %zu bytes", name, need);
+    LSSM_REQUIRE((uintptr_t)ws % 16 == 0, "%s: the workspace must be 16-byte aligned", name);
+    SsdBwdArgs a{};
+    a.X = X;
+    a.B = B;
+    a.C = C;
+    a.dt = dt_raw;
+    a.dt_bias = dt_bias;
+    a.A_log = A_log;
+    a.D = d.has_D ? D_skip : nullptr;
+    a.state = state;
+    a.dY = dY;
+    a.d_state = d_state;
+    a.dX = dX;
+    a.dB = dB;
+    a.dC = dC;
+    a.d_dt = d_dt;
+    a.d_dt_bias = d_dt_bias;
+    a.dA_log = dA_log;
+    a.dD = d.has_D ? dD : nullptr;
+    a.d_state0 = d_state0;
+    a.batch = batch;
+    a.L = d.L;
+    a.H = d.H;
+    a.P = d.P;
+    a.N = d.N;
+    a.G = d.n_groups;
+    a.dt_min = d.dt_min;
+    a.dt_max = d.dt_max;
+    hipError_t e = launch_ssd_bwd(ctx->stream, a, d, act, ws);
+    if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
+    return finish(ctx, name);
+}
+
 int lssm_ssd_step(lssm_ctx* ctx, const void* x, const void* B, const void* C, const void* dt_raw,
                   const void* dt_bias, const void* A_log, const void* D_skip, float* state, void* y,
                   uint32_t batch, lssm_ssd_step_dims d, lssm_dtype act) {

@@ -229,6 +229,7 @@ static const char* const kKernelNames[] = {
     "argmax",
     "token_logprobs",
     "token_logprobs_bwd",
+    "ssd_chunked_bwd",
 };
 
 int lssm_kernel_count(void) { return (int)(sizeof(kKernelNames) / sizeof(kKernelNames[0])); }

@@ -164,6 +164,26 @@ hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws);
 // the gradient alone, from kept statistics
 hipError_t launch_logprobs_grad(hipStream_t s, LogprobArgs a, int act);
 
+// Gradients of the chunked scan (ssd_bwd.hip), packed rows.
+struct SsdBwdArgs {
+    const void *X, *B, *C, *dt, *dt_bias, *A_log, *D;   // as SsdArgs; D null: none
+    const float* state;                                 // entering the scan, or null: zero
+    const void* dY;
+    const float* d_state;                               // of the state that leaves it, or null: zero
+    void *dX, *dB, *dC, *d_dt, *d_dt_bias, *dA_log, *dD;
+    float* d_state0;                                    // or null
+    uint32_t batch, L, H, P, N, G;
+    float dt_min, dt_max;
+    // set by the launcher
+    uint32_t nchunk, nslice, nsplit;
+    float *hst, *gst;       // [batch][H][chunk][P][N]: h0 and G1 of every chunk
+    float *bpart, *cpart;   // [share][batch][L][G][N]
+    float* q;               // [slice][batch][H][L]: gradient of dt
+    float* part;            // [batch][H][slice][chunk][2]: sums of dA_log and dD
+};
+size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act);
+hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, int act, void* ws);
+
 // appends next[0..B) as row *pos of log [cap][B] and advances *pos (B <= 64)
 hipError_t launch_id_log(hipStream_t s, const int32_t* next, uint32_t B, int32_t* log, uint32_t cap,
                          uint32_t* pos);
