@@ -180,6 +180,7 @@ struct SsdBwdArgs {
     float *bpart, *cpart;   // [share][batch][L][G][N]
     float* q;               // [slice][batch][H][L]: gradient of dt
     float* part;            // [batch][H][slice][chunk][2]: sums of dA_log and dD
+    float *lc, *dtv;        // bf16 form: [batch][H][chunk][token]: sums of A dt, dt
 };
 size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act);
 hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, int act, void* ws);

@@ -326,6 +326,569 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
 }
 
 // ---------------------------------------------------------------------------
+// bf16, N = 128, P a multiple of 64: chunks of 128 tokens, slices of 64 state
+// rows, v_mfma_f32_16x16x32_bf16.  An operand formed in fp32 (weighted rows,
+// states, M, the heads' sum of S) enters as a sum of bf16 pieces, each the
+// rounding of what the pieces before it left: two pieces hold it to 2^-17,
+// three to 2^-25.  What an operand of 16 bits holds already is exact.
+// The 16x16x32 operands: lane l = 16 q + i supplies row / column i, k = 8 q ..
+// 8 q + 7; the result holds rows 4 q .. 4 q + 3 of column i.  Operands whose k
+// runs down the rows of a tile are read with the transposing LDS load.
+// ---------------------------------------------------------------------------
+constexpr int FQ = 128;      // tokens a chunk
+constexpr int FP = 64;       // state rows a slice
+constexpr int FN = 128;      // state size
+constexpr int FXP = FP + 8;  // pitch of a [token or n][row] tile
+constexpr int FBP = FN + 8;  // pitch of a [token][n] tile
+constexpr int F_NT = 512;
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef short s8v __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// LDS traffic only: global loads and stores stay in flight across it
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ floatx4 mma(s8v a, s8v b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// lane i of each 16 lanes: column i of four rows, one row of each four lanes
+__device__ __forceinline__ s4v ld_tr(const bf16* p) {
+    typedef __attribute__((address_space(3))) s4v lds_s4v;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v*)(const_cast<bf16*>(p)));
+}
+__device__ __forceinline__ s8v cat8(s4v lo, s4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ float val(short b) { return __uint_as_float((uint32_t)(uint16_t)b << 16); }
+
+// v rounded to bf16; v becomes what is left
+__device__ __forceinline__ s4v take4(floatx4& v) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, bf16x2));
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, bf16x2));
+    v[0] -= __uint_as_float(a << 16);
+    v[1] -= __uint_as_float(a & 0xffff0000u);
+    v[2] -= __uint_as_float(b << 16);
+    v[3] -= __uint_as_float(b & 0xffff0000u);
+    return __builtin_bit_cast(s4v, u32x2{a, b});
+}
+
+// dt and the sums of A dt of every chunk, zeros and the last sum behind the
+// end: block (chunk, head, sequence), a thread a token
+__global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
+    __shared__ double s[FQ];
+    const uint32_t c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
+    const double A = -exp((double)to_f(((const bf16*)a.A_log)[h]));
+    float dt = 0.0f;
+    if (c * FQ + t < a.L) {
+        const float v = to_f(((const bf16*)a.dt)[((size_t)b * a.L + c * FQ + t) * a.H + h]) + to_f(((const bf16*)a.dt_bias)[h]);
+        dt = v > 20.0f ? v : log1pf(expf(v));
+        dt = fminf(fmaxf(dt, a.dt_min), a.dt_max);
+    }
+    s[t] = A * (double)dt;
+    __syncthreads();
+    for (int d = 1; d < FQ; d <<= 1) {
+        const double o = (int)t >= d ? s[t - d] : 0.0;
+        __syncthreads();
+        s[t] += o;
+        __syncthreads();
+    }
+    const size_t at = (((size_t)b * a.H + h) * a.nchunk + c) * FQ + t;
+    a.lc[at] = (float)s[t];
+    a.dtv[at] = dt;
+}
+
+// 16-byte piece i of a tile of FQ rows, `per` pieces a row: zeros behind the
+// rows there are
+__device__ __forceinline__ u32x4 piece(const bf16* src, size_t stride, uint32_t rows, uint32_t per, uint32_t i) {
+    const uint32_t r = i / per, c = i % per;
+    return r < rows ? *reinterpret_cast<const u32x4*>(src + r * stride + 8 * c) : u32x4{0, 0, 0, 0};
+}
+
+// The walk: block (head, slice), sequence, direction; wave (pt, nh) keeps the
+// state's rows 16 pt .. + 15 and columns 64 nh .. + 63 in fp32.  A chunk's
+// state goes out as two pieces, [piece][n][row], the order in which the
+// chunks' kernel takes it as an operand.
+__global__ __launch_bounds__(F_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
+    __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * FBP];
+    __shared__ __attribute__((aligned(16))) float W[FQ];
+    __shared__ float Dq;
+    const uint32_t h = blockIdx.x / a.nslice, sl = blockIdx.x % a.nslice, b = blockIdx.y;
+    const bool back = blockIdx.z != 0;
+    const uint32_t P = a.P, L = a.L, g = h / (a.H / a.G), tid = threadIdx.x;
+    const int lane = tid % WAVE, li = lane % 16, lq = lane / 16, tk = li / 4, tc = li % 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE), pt = w % 4, nh = w / 4;
+    const float* init = back ? a.d_state : a.state;
+    bf16* slots = (bf16*)(back ? a.gst : a.hst) + (((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk * (2 * FN * FP);
+    const bf16* rows = (const bf16*)(back ? a.dY : a.X) + (size_t)b * L * a.H * P + (size_t)h * P + sl * FP;
+    const bf16* cols = (const bf16*)(back ? a.C : a.B) + (size_t)b * L * a.G * FN + (size_t)g * FN;
+    const float* lc = a.lc + ((size_t)b * a.H + h) * a.nchunk * FQ;
+    const float* dtv = a.dtv + ((size_t)b * a.H + h) * a.nchunk * FQ;
+    const size_t plain = (((size_t)b * a.H + h) * P + sl * FP + 16 * pt + 4 * lq) * FN + 64 * nh + li;
+
+    floatx4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[i][r] = init ? init[plain + r * FN + 16 * i] : 0.0f;
+
+    u32x4 rx[2], rb[4];
+    float rl = 0.0f, rt = 0.0f, rd = 0.0f;
+    auto fetch = [&](uint32_t c) {
+        const uint32_t t0 = c * FQ, tl = min((uint32_t)FQ, L - t0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) rx[i] = piece(rows + (size_t)t0 * a.H * P, (size_t)a.H * P, tl, FP / 8, tid + i * F_NT);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rb[i] = piece(cols + (size_t)t0 * a.G * FN, (size_t)a.G * FN, tl, FN / 8, tid + i * F_NT);
+        rl = lc[t0 + tid % FQ];
+        rt = lc[t0 + FQ - 1];
+        rd = dtv[t0 + tid % FQ];
+    };
+    const uint32_t first = back ? a.nchunk - 1 : 0;
+    if (a.nchunk) fetch(first);
+    for (uint32_t k = 0; k < a.nchunk; ++k) {
+        const uint32_t c = back ? a.nchunk - 1 - k : k;
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t j = tid + i * F_NT;
+            *reinterpret_cast<u32x4*>(Xs + j / (FP / 8) * FXP + j % (FP / 8) * 8) = rx[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t j = tid + i * F_NT;
+            *reinterpret_cast<u32x4*>(Bs + j / (FN / 8) * FBP + j % (FN / 8) * 8) = rb[i];
+        }
+        if (tid < FQ) W[tid] = back ? __expf(rl) : rd * __expf(rt - rl);
+        if (tid == 0) Dq = __expf(rt);
+        lds_barrier();
+        if (k + 1 < a.nchunk) fetch(back ? c - 1 : c + 1);
+        bf16* slot = slots + (size_t)c * (2 * FN * FP);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            bf16* o = slot + (64 * nh + 16 * i + li) * FP + 16 * pt + 4 * lq;
+            floatx4 v = s[i];
+            *reinterpret_cast<s4v*>(o) = take4(v);
+            *reinterpret_cast<s4v*>(o + FN * FP) = take4(v);
+        }
+        const float dq = Dq;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] *= dq;
+#pragma unroll
+        for (int ks = 0; ks < FQ / 32; ++ks) {
+            const bf16* xp = Xs + (32 * ks + 8 * lq + tk) * FXP + 16 * pt + 4 * tc;
+            const s4v x0 = ld_tr(xp), x1 = ld_tr(xp + 4 * FXP);
+            floatx4 v0 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq);
+            floatx4 v1 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v0[e] *= val(x0[e]);
+                v1[e] *= val(x1[e]);
+            }
+            // three pieces: the gradient of the first state is given in fp32
+            s8v f[3];
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                const s4v lo = take4(v0);
+                f[e] = cat8(lo, take4(v1));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bf16* bp = Bs + (32 * ks + 8 * lq + tk) * FBP + 64 * nh + 16 * i + 4 * tc;
+                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 4 * FBP));
+#pragma unroll
+                for (int e = 0; e < 3; ++e) s[i] = mma(f[e], bt, s[i]);
+            }
+        }
+    }
+    if (back && a.d_state0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a.d_state0[plain + r * FN + 16 * i] = s[i][r];
+}
+
+// The chunks' gradients: block = chunk, sequence, group, share of the group's
+// (head, slice) pairs, which it takes one after the other.  Wave w
+//   - keeps dB and dC of state columns 16 w .. + 15, all tokens, in registers;
+//   - forms column J of S and M (source tokens 16 J .. + 15, all sinks), J such
+//     that the two waves of a SIMD share nine of the 36 lower tiles, and from
+//     it dx of those tokens; M goes from the registers that S came out in
+//     into the next product.
+// C B^T and the heads' sum of S (lower tiles, as their product leaves them) live
+// in LDS.  The next pair's rows and states are on their way into registers
+// while this one is worked on.
+constexpr int F_TILES = 36;
+__device__ __forceinline__ constexpr int tile_of(int T, int J) { return T * (T + 1) / 2 + J; }
+
+__global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) {
+    __shared__ __attribute__((aligned(16))) bf16 stage[4 * FQ * FXP];
+    __shared__ __attribute__((aligned(16))) floatx4 SS[F_TILES * WAVE], CB[F_TILES * WAVE];
+    __shared__ __attribute__((aligned(16))) float LC[FQ], DT[FQ], EL[FQ], ER[FQ], WB[FQ], AF[FQ];
+    __shared__ float VO[8][FQ], RS[8][FQ], UO[FQ], CS[FQ], red[8][2];
+    bf16 *Xs = stage, *Ys = stage + FQ * FXP, *Gh = stage + 2 * FQ * FXP, *Gl = stage + 3 * FQ * FXP;
+    const uint32_t P = a.P, L = a.L, hpg = a.H / a.G;
+    uint32_t tid = threadIdx.x;
+    const uint32_t c = blockIdx.x % a.nchunk, sp = blockIdx.x / a.nchunk % a.nsplit;
+    const uint32_t g = blockIdx.x / a.nchunk / a.nsplit, b = blockIdx.y;
+    const uint32_t t0 = c * FQ, tl = min((uint32_t)FQ, L - t0);
+    int lane = tid % WAVE, li = lane % 16, lq = lane / 16, tk = li / 4, tc = li % 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int J = w < 4 ? w : 11 - w;
+    const size_t hp = (size_t)a.H * P, gn = (size_t)a.G * FN;
+    const bf16* Bg = (const bf16*)a.B + ((size_t)b * L + t0) * gn + (size_t)g * FN;
+    const bf16* Cg = (const bf16*)a.C + ((size_t)b * L + t0) * gn + (size_t)g * FN;
+
+    const uint32_t pairs = hpg * a.nslice, per = (pairs + a.nsplit - 1) / a.nsplit;
+    const uint32_t v_first = sp * per, v_end = min(pairs, v_first + per);
+    u32x4 rx[2], ry[2], rg[4], rh[4];
+    float rl = 0.0f, rt = 0.0f, rr = 0.0f, rd = 0.0f;
+    auto fetch = [&](uint32_t v) {
+        const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
+        const size_t row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            rx[i] = piece((const bf16*)a.X + row0, hp, tl, FP / 8, tid + i * F_NT);
+            ry[i] = piece((const bf16*)a.dY + row0, hp, tl, FP / 8, tid + i * F_NT);
+        }
+        const size_t slot = ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * (2 * FN * FP);
+        const bf16 *gs = (const bf16*)a.gst + slot, *hs = (const bf16*)a.hst + slot;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            rg[i] = *reinterpret_cast<const u32x4*>(gs + 8 * (size_t)(tid + i * F_NT));
+            rh[i] = *reinterpret_cast<const u32x4*>(hs + (i / 2) * (FN * FP) + (16 * w + li) * FP + 32 * (i % 2) + 8 * lq);
+        }
+        const float* lc = a.lc + (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
+        const uint32_t t = tid % FQ;
+        rl = lc[t];
+        rt = lc[FQ - 1];
+        rr = t >= 16 ? lc[t / 16 * 16 - 1] : 0.0f;
+        rd = a.dtv[(((size_t)b * a.H + h) * a.nchunk + c) * FQ + t];
+    };
+
+    // C B^T, lower tiles
+    auto row8 = [&](const bf16* p, uint32_t t, int at) {
+        return t < tl ? *reinterpret_cast<const s8v*>(p + t * gn + at) : s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    };
+    for (int i = w; i < F_TILES; i += 8) {
+        int T = 0;
+        while (tile_of(T + 1, 0) <= i) ++T;
+        const int Jc = i - tile_of(T, 0);
+        floatx4 acc{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < FN / 32; ++ks)
+            acc = mma(row8(Cg, 16 * T + li, 32 * ks + 8 * lq), row8(Bg, 16 * Jc + li, 32 * ks + 8 * lq), acc);
+        CB[i * WAVE + lane] = acc;
+        SS[i * WAVE + lane] = floatx4{0, 0, 0, 0};
+    }
+    RS[w][lane] = RS[w][lane + 64] = 0.0f;      // sinks before the wave's sources stay 0
+    s8v bf[4];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) bf[ks] = row8(Bg, 16 * J + li, 32 * ks + 8 * lq);
+    u32x2 cp[8];                                 // C[t = 16 T + 4 lq + r][n = 16 w + li]
+#pragma unroll
+    for (int T = 0; T < 8; ++T)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            uint32_t x = 0;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const uint32_t t = 16 * T + 4 * lq + 2 * k + r;
+                if (t < tl) x |= (uint32_t)*reinterpret_cast<const uint16_t*>(Cg + t * gn + 16 * w + li) << (16 * r);
+            }
+            cp[T][k] = x;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+    floatx4 dc[8], db[8];
+#pragma unroll
+    for (int T = 0; T < 8; ++T) dc[T] = db[T] = floatx4{0, 0, 0, 0};
+    if (v_first < v_end) fetch(v_first);
+
+    for (uint32_t v = v_first; v < v_end; ++v) {
+        const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
+        // places and C's values are formed again for each pair: kept over the
+        // loop they would push what has to be kept out of the registers
+        asm volatile("" : "+v"(tid), "+v"(lane), "+v"(li), "+v"(lq), "+v"(tk), "+v"(tc));
+#pragma unroll
+        for (int T = 0; T < 8; ++T) asm volatile("" : "+v"(cp[T]));
+        lds_barrier();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t j = tid + i * F_NT, at = j / (FP / 8) * FXP + j % (FP / 8) * 8;
+            *reinterpret_cast<u32x4*>(Xs + at) = rx[i];
+            *reinterpret_cast<u32x4*>(Ys + at) = ry[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t j = (tid + i * F_NT) % (FN * FP / 8);
+            *reinterpret_cast<u32x4*>((i < 2 ? Gh : Gl) + j / (FP / 8) * FXP + j % (FP / 8) * 8) = rg[i];
+        }
+        if (tid < FQ) {
+            const float er = __expf(rt - rl);
+            LC[tid] = rl;
+            DT[tid] = rd;
+            EL[tid] = __expf(rl);
+            ER[tid] = er;
+            WB[tid] = rd * er;
+            AF[tid] = __expf(rl - rr);
+        }
+        lds_barrier();
+
+        // dB: x and G1 (k = row)
+        s8v gf[4], hf[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            gf[i] = *reinterpret_cast<const s8v*>((i / 2 ? Gl : Gh) + (16 * w + li) * FXP + 32 * (i % 2) + 8 * lq);
+            hf[i] = __builtin_bit_cast(s8v, rh[i]);
+        }
+        float gh = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                gh = fmaf(val(gf[i][e]) + val(gf[i + 2][e]), val(hf[i][e]) + val(hf[i + 2][e]), gh);
+        gh = wave_sum(gh);
+#pragma unroll
+        for (int T = 0; T < 8; ++T) {
+            const bf16* xp = Xs + (16 * T + li) * FXP + 8 * lq;
+            const s8v x0 = *reinterpret_cast<const s8v*>(xp), x1 = *reinterpret_cast<const s8v*>(xp + 32);
+            floatx4 y{0, 0, 0, 0};
+            y = mma(x0, gf[0], y);
+            y = mma(x1, gf[1], y);
+            y = mma(x0, gf[2], y);
+            y = mma(x1, gf[3], y);
+            const floatx4 wb = *reinterpret_cast<const floatx4*>(WB + 16 * T + 4 * lq);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) db[T][r] = fmaf(wb[r], y[r], db[T][r]);
+            if (T % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // dx'^T [row][source] from G1 and B (k = n)
+        const int j = 16 * J + li;
+        floatx4 dx[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) dx[p] = floatx4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const int at = (32 * ks + 8 * lq + tk) * FXP + 16 * p + 4 * tc;
+                dx[p] = mma(cat8(ld_tr(Gh + at), ld_tr(Gh + at + 4 * FXP)), bf[ks], dx[p]);
+                dx[p] = mma(cat8(ld_tr(Gl + at), ld_tr(Gl + at + 4 * FXP)), bf[ks], dx[p]);
+                if (p % 2) __builtin_amdgcn_sched_barrier(0);
+            }
+        const float erj = ER[j], dtj = DT[j], lcj = LC[j];
+        float uo = 0.0f;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const s4v x = *reinterpret_cast<const s4v*>(Xs + j * FXP + 16 * p + 4 * lq);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                dx[p][r] *= erj;
+                uo = fmaf(dx[p][r], val(x[r]), uo);
+            }
+        }
+        uo = swap_add32(swap_add16(uo));
+
+        // sinks T: dC of all sources before the chunk; S and M of column J
+        const s8v xj0 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 8 * lq);
+        const s8v xj1 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 32 + 8 * lq);
+        float col = 0.0f, diag = 0.0f;
+#pragma unroll
+        for (int T2 = 0; T2 < 8; T2 += 2) {
+            s4v mh[2], ml[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int T = T2 + k;
+                const bf16* yp = Ys + (16 * T + li) * FXP + 8 * lq;
+                const s8v y0 = *reinterpret_cast<const s8v*>(yp), y1 = *reinterpret_cast<const s8v*>(yp + 32);
+                floatx4 x{0, 0, 0, 0};
+                x = mma(y0, hf[0], x);
+                x = mma(y1, hf[1], x);
+                x = mma(y0, hf[2], x);
+                x = mma(y1, hf[3], x);
+                const floatx4 el = *reinterpret_cast<const floatx4*>(EL + 16 * T + 4 * lq);
+                floatx4 vo;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float d = el[r] * x[r];
+                    dc[T][r] += d;
+                    vo[r] = group_sum<16>(d * __uint_as_float(r & 1 ? cp[T][r / 2] & 0xffff0000u : cp[T][r / 2] << 16));
+                }
+                if (li == 0) *reinterpret_cast<floatx4*>(&VO[w][16 * T + 4 * lq]) = vo;
+                mh[k] = ml[k] = s4v{0, 0, 0, 0};
+                if (T >= J) {
+                    floatx4 sd{0, 0, 0, 0};
+                    sd = mma(y0, xj0, sd);
+                    sd = mma(y1, xj1, sd);
+                    const int id = tile_of(T, 0) + J;
+                    floatx4 e;
+                    if (T > J) {
+                        const float f = __expf(LC[16 * T - 1] - lcj);
+                        e = *reinterpret_cast<const floatx4*>(AF + 16 * T + 4 * lq) * f;
+                    } else {
+                        const floatx4 lt = *reinterpret_cast<const floatx4*>(LC + 16 * T + 4 * lq);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            e[r] = 4 * lq + r >= li ? __expf(lt[r] - lcj) : 0.0f;
+                            diag += 4 * lq + r == li ? sd[r] : 0.0f;
+                        }
+                    }
+                    const floatx4 cb = CB[id * WAVE + lane];
+                    floatx4 ss = SS[id * WAVE + lane], m, row;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        m[r] = cb[r] * e[r];
+                        ss[r] = fmaf(sd[r] * e[r], dtj, ss[r]);
+                        const float kk = sd[r] * m[r];
+                        col += kk;
+                        row[r] = group_sum<16>(kk * dtj);
+                    }
+                    SS[id * WAVE + lane] = ss;
+                    if (li == 0) *reinterpret_cast<floatx4*>(&RS[w][16 * T + 4 * lq]) = row;
+                    mh[k] = take4(m);
+                    ml[k] = take4(m);
+                }
+            }
+            if (T2 + 1 >= J) {
+                const s8v h8 = cat8(mh[0], mh[1]), l8 = cat8(ml[0], ml[1]);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const bf16* yp = Ys + (16 * T2 + 4 * lq + tk) * FXP + 16 * p + 4 * tc;
+                    const s8v yt = cat8(ld_tr(yp), ld_tr(yp + 16 * FXP));
+                    dx[p] = mma(yt, h8, dx[p]);
+                    dx[p] = mma(yt, l8, dx[p]);
+                }
+            }
+        }
+        if (v + 1 < v_end) fetch(v + 1);
+        col = swap_add32(swap_add16(col));
+        if (lq == 0) {
+            UO[j] = uo;
+            CS[j] = col;
+        }
+        diag = wave_sum(diag);
+        if (lane == 0) {
+            red[w][0] = gh;
+            red[w][1] = diag;
+        }
+        const float D = a.D ? to_f(((const bf16*)a.D)[h]) : 0.0f;
+        bf16* out = (bf16*)a.dX + ((size_t)b * L + t0 + j) * hp + (size_t)h * P + sl * FP;
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const s4v y = *reinterpret_cast<const s4v*>(Ys + j * FXP + 16 * p + 4 * lq);
+            floatx4 o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(dtj, dx[p][r], D * val(y[r]));
+            if (j < (int)tl) *reinterpret_cast<s4v*>(out + 16 * p + 4 * lq) = take4(o);
+        }
+        lds_barrier();
+        // a_t: pairs of a source before t and a sink from t on; lane l has
+        // tokens 2 l and 2 l + 1
+        if (w == 7) {
+            float pre[2], suf[2], dir[2], dt[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int t = 2 * lane + k;
+                float s = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += VO[i][t];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += RS[i][t];
+                dt[k] = DT[t];
+                dir[k] = UO[t] + CS[t];
+                pre[k] = dt[k] * UO[t];
+                suf[k] = s - dt[k] * CS[t];
+            }
+            const float both = pre[0] + pre[1], own = suf[0] + suf[1];
+            const float p_in = wave_prefix_sum(both) - both;
+            const float s_all = wave_sum(own), s_from = s_all - wave_prefix_sum(own);   // behind this lane's
+            float e0 = 0.0f, dd = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e0 += red[i][0];
+                dd += red[i][1];
+            }
+            const float edge = __expf(LC[FQ - 1]) * e0, A = -expf(to_f(((const bf16*)a.A_log)[h]));
+            float da[2];
+            da[0] = edge + p_in + (s_from + own);
+            da[1] = edge + (p_in + pre[0]) + (s_from + suf[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (2 * lane + k < (int)tl)
+                    a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + 2 * lane + k] = dir[k] + A * da[k];
+            const float dA = wave_sum(dt[0] * da[0] + dt[1] * da[1]);
+            if (lane == 0) {
+                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 2;
+                o[0] = A * dA;
+                o[1] = dd;
+            }
+        }
+    }
+
+    // within the chunk: sum of S over the share's heads with B and C
+    lds_barrier();
+    bf16 *Bs = stage, *Cs = stage + FQ * FBP;
+    static_assert(2 * FBP <= 4 * FXP, "B and C fit where the pairs' tiles were");
+    for (uint32_t i = tid; i < FQ * FN / 8; i += F_NT) {
+        *reinterpret_cast<u32x4*>(Bs + i / (FN / 8) * FBP + i % (FN / 8) * 8) = piece(Bg, gn, tl, FN / 8, i);
+        *reinterpret_cast<u32x4*>(Cs + i / (FN / 8) * FBP + i % (FN / 8) * 8) = piece(Cg, gn, tl, FN / 8, i);
+    }
+    lds_barrier();
+    const float* Sf = reinterpret_cast<const float*>(SS);
+#pragma unroll
+    for (int T = 0; T < 8; ++T) {
+        // dB of source tile T: sinks k = T ..; dC of sink tile T: sources k = .. T
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+            const bf16* tp = (Cs + (16 * k + 4 * lq + tk) * FBP + 16 * w + 4 * tc);
+            if (k + 1 >= T) {
+                s4v hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    floatx4 x{0, 0, 0, 0};
+                    if (k + e >= T) x = SS[(tile_of(k + e, 0) + T) * WAVE + lane];
+                    hi[e] = take4(x);
+                    lo[e] = take4(x);
+                }
+                const s8v ct = cat8(ld_tr(tp), ld_tr(tp + 16 * FBP));
+                db[T] = mma(cat8(hi[0], hi[1]), ct, db[T]);
+                db[T] = mma(cat8(lo[0], lo[1]), ct, db[T]);
+            }
+            if (k <= T) {
+                const bf16* bp = (Bs + (16 * k + 4 * lq + tk) * FBP + 16 * w + 4 * tc);
+                s4v hi[2], lo[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    floatx4 x{0, 0, 0, 0};
+                    if (k + e <= T)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            x[r] = Sf[((tile_of(T, 0) + k + e) * WAVE + 4 * lq + r + 16 * tk) * 4 + tc];
+                    hi[e] = take4(x);
+                    lo[e] = take4(x);
+                }
+                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 16 * FBP));
+                dc[T] = mma(cat8(hi[0], hi[1]), bt, dc[T]);
+                dc[T] = mma(cat8(lo[0], lo[1]), bt, dc[T]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t t = 16 * T + 4 * lq + r;
+            if (t < tl) {
+                const size_t at = ((((size_t)sp * a.batch + b) * L + t0 + t) * a.G + g) * FN + 16 * w + li;
+                a.cpart[at] = dc[T][r];
+                a.bpart[at] = db[T][r];
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Sums over shares, slices and chunks
 // ---------------------------------------------------------------------------
 // gradient of raw + bias from that of dt: the softplus' slope, 0 where the
@@ -394,27 +957,43 @@ template <typename F> hipError_t with_type(int act, F f) {
     return f(float{});
 }
 
-// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts]
+// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts][steps]
 struct Plan {
+    bool fast;
     uint32_t nchunk, nslice, nsplit;
-    size_t states, rows, q, part;      // floats of one of each
-    size_t floats() const { return 2 * states + 2 * rows + q + part; }
+    size_t states, rows, q, part, steps;      // floats of one of each
+    size_t floats() const { return 2 * states + 2 * rows + q + part + 2 * steps; }
 };
-Plan plan_of(uint32_t batch, const lssm_ssd_dims& d) {
+Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     Plan p;
-    p.nchunk = (d.L + GQ - 1) / GQ;
-    p.nslice = (d.P + GP - 1) / GP;
+    p.fast = fast;
+    const uint32_t qn = fast ? FQ : GQ, rn = fast ? FP : GP;
+    p.nchunk = (d.L + qn - 1) / qn;
+    p.nslice = (d.P + rn - 1) / rn;
+    // shares of a group's (head, slice) pairs: the fewest rounds of blocks
+    // over the chip, a block's own work taken as two pairs more
     const uint32_t pairs = d.H / d.n_groups * p.nslice;
-    // shares of a group's heads: two blocks a CU where there are that many
-    const size_t blocks = std::max<size_t>(1, (size_t)p.nchunk * batch * d.n_groups);
-    p.nsplit = (uint32_t)std::min<size_t>(pairs, (512 + blocks - 1) / blocks);
-    p.nsplit = (pairs + (pairs + p.nsplit - 1) / p.nsplit - 1) / ((pairs + p.nsplit - 1) / p.nsplit);
+    const size_t blocks = std::max<size_t>(1, (size_t)p.nchunk * batch * d.n_groups), cus = (fast ? 1 : 2) * (size_t)num_cus();
+    size_t best = 0;
+    p.nsplit = 1;
+    for (uint32_t per = pairs; per >= 1; --per) {
+        const uint32_t n = (pairs + per - 1) / per;
+        const size_t cost = (blocks * n + cus - 1) / cus * (per + 2);
+        if (per == pairs || cost < best) {
+            best = cost;
+            p.nsplit = n;
+        }
+    }
     p.states = (size_t)batch * d.H * p.nchunk * d.P * d.N;
     p.rows = (size_t)p.nsplit * batch * d.L * d.n_groups * d.N;
     p.q = (size_t)p.nslice * batch * d.H * d.L;
     p.part = (size_t)batch * d.H * p.nslice * p.nchunk * 2;
+    p.steps = fast ? (size_t)batch * d.H * p.nchunk * FQ : 0;
+    // every array starts on a 16-byte address
+    for (size_t* n : {&p.states, &p.rows, &p.q, &p.part, &p.steps}) *n = (*n + 3) / 4 * 4;
     return p;
 }
+bool fast_dims(const lssm_ssd_dims& d, int act) { return act == LSSM_BF16 && d.N == FN && d.P % FP == 0; }
 
 template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArgs& a) {
     ssd_bwd_walk_kernel<T, NT><<<dim3(a.H * a.nslice, a.batch, 2), G_NT, 0, s>>>(a);
@@ -424,13 +1003,17 @@ template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArg
 
 }  // namespace
 
+// (the larger of both plans: alignment of the arrays decides at the call)
 size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act) {
-    (void)act;
-    return plan_of(batch, d).floats() * sizeof(float);
+    size_t n = plan_of(batch, d, false).floats();
+    if (fast_dims(d, act)) n = std::max(n, plan_of(batch, d, true).floats());
+    return n * sizeof(float);
 }
 
 hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, int act, void* ws) {
-    const Plan p = plan_of(a.batch, d);
+    bool fast = fast_dims(d, act);
+    for (const void* p : {a.X, a.B, a.C, a.dY, (const void*)a.dX}) fast = fast && (uintptr_t)p % 16 == 0;
+    const Plan p = plan_of(a.batch, d, fast);
     a.nchunk = p.nchunk;
     a.nslice = p.nslice;
     a.nsplit = p.nsplit;
@@ -440,10 +1023,17 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
     a.cpart = a.bpart + p.rows;
     a.q = a.cpart + p.rows;
     a.part = a.q + p.q;
+    a.lc = a.part + p.part;
+    a.dtv = a.lc + p.steps;
     return with_type(act, [&](auto z) {
         using T = decltype(z);
         if (a.batch) {
-            if (a.N <= 64) launch_generic<T, 64>(s, a);
+            if (fast) {
+                if (a.nchunk) ssd_bwd_steps_kernel<<<dim3(a.nchunk, a.H, a.batch), FQ, 0, s>>>(a);
+                ssd_bwd_walk_bf16_kernel<<<dim3(a.H * a.nslice, a.batch, 2), F_NT, 0, s>>>(a);
+                if (a.nchunk)
+                    ssd_bwd_chunk_bf16_kernel<<<dim3(a.nchunk * a.nsplit * a.G, a.batch), F_NT, 0, s>>>(a);
+            } else if (a.N <= 64) launch_generic<T, 64>(s, a);
             else if (a.N <= 128) launch_generic<T, 128>(s, a);
             else launch_generic<T, 256>(s, a);
             const size_t n = (size_t)a.batch * a.L * std::max(a.G * a.N, a.H);
