@@ -177,10 +177,12 @@ struct SsdBwdArgs {
     // set by the launcher
     uint32_t nchunk, nslice, nsplit;
     float *hst, *gst;       // [batch][H][chunk][P][N]: h0 and G1 of every chunk
-    float *bpart, *cpart;   // [share][batch][L][G][N]
-    float* q;               // [slice][batch][H][L]: gradient of dt
-    float* part;            // [batch][H][slice][chunk][2]: sums of dA_log and dD
-    float *lc, *dtv;        // bf16 form: [batch][H][chunk][token]: sums of A dt, dt
+    float *bpart, *cpart;   // [share][batch][L][G][N], `share` floats a share
+    float* q;               // [slice][batch][H][L]: gradient of dt_raw
+    float* part;            // [batch][H][slice][chunk][3]: sums of d_dt_bias, dA_log and dD
+    float *lc, *dtv, *slope;   // bf16 form: [batch][H][chunk][token]: sums of A dt, dt, d dt / d raw
+    size_t share;
+    uint32_t row_blocks, dt_blocks;
 };
 size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act);
 hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, int act, void* ws);

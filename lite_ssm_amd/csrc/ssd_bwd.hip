@@ -53,6 +53,14 @@ constexpr int GP = 32;      // state rows a slice
 constexpr int GXP = 36;     // LDS pitch of a [token][row] tile (= 4 modulo 64 banks x 9)
 constexpr int G_NT = 256;
 
+// gradient of raw + bias from that of dt: the softplus' slope, 0 where the
+// clamp holds
+template <typename T> __device__ __forceinline__ float dt_slope(const SsdBwdArgs& a, uint32_t b, uint32_t t, uint32_t h) {
+    const float v = to_f(((const T*)a.dt)[((size_t)b * a.L + t) * a.H + h]) + to_f(((const T*)a.dt_bias)[h]);
+    const float sp = v > 20.0f ? v : log1pf(expf(v));
+    return sp >= a.dt_min && sp <= a.dt_max ? 1.0f / (1.0f + expf(-v)) : 0.0f;
+}
+
 struct Steps { double lc, tot; float dt; };
 
 // dt and the sums of A dt of a chunk of GQ tokens, lane t of a wave (lanes
@@ -289,12 +297,18 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
             const float edge = (float)exp(tot) * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
             const float da = edge + (pre - own) + suf;
             const float A = -expf(to_f(((const T*)a.A_log)[h]));
-            if (lane < (int)tl) a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + lane] = uo + cs + A * da;
+            float q = 0.0f;
+            if (lane < (int)tl) {
+                q = (uo + cs + A * da) * dt_slope<T>(a, b, t0 + lane, h);
+                a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + lane] = q;
+            }
             const float dA = wave_sum(dt * da);
+            q = wave_sum(q);
             if (lane == 0) {
-                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 2;
-                o[0] = A * dA;
-                o[1] = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
+                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 3;
+                o[0] = q;
+                o[1] = A * dA;
+                o[2] = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
             }
         }
     }
@@ -303,7 +317,7 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
 #pragma unroll
     for (int r = 0; r < 4; ++r) Ms[(16 * T0 + 4 * lq + r) * GXP + 16 * J0 + li] = ssum[r];
     __syncthreads();
-    const size_t base = (size_t)sp * a.batch * L * a.G * N;
+    const size_t base = (size_t)sp * a.share;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -361,6 +375,11 @@ __device__ __forceinline__ s4v ld_tr(const bf16* p) {
 __device__ __forceinline__ s8v cat8(s4v lo, s4v hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ float val(short b) { return __uint_as_float((uint32_t)(uint16_t)b << 16); }
 
+// a buffer of `bytes` from p on: loads past its end give 0
+__device__ __forceinline__ auto rsrc(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+}
+
 // v rounded to bf16; v becomes what is left
 __device__ __forceinline__ s4v take4(floatx4& v) {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -397,6 +416,7 @@ __global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
     const size_t at = (((size_t)b * a.H + h) * a.nchunk + c) * FQ + t;
     a.lc[at] = (float)s[t];
     a.dtv[at] = dt;
+    a.slope[at] = c * FQ + t < a.L ? dt_slope<bf16>(a, b, c * FQ + t, h) : 0.0f;
 }
 
 // 16-byte piece i of a tile of FQ rows, `per` pieces a row: zeros behind the
@@ -463,7 +483,14 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
         if (tid < FQ) W[tid] = back ? __expf(rl) : rd * __expf(rt - rl);
         if (tid == 0) Dq = __expf(rt);
         lds_barrier();
-        if (k + 1 < a.nchunk) fetch(back ? c - 1 : c + 1);
+        if (k + 1 < a.nchunk) {
+            fetch(back ? c - 1 : c + 1);
+        } else {
+            // (not kept over the loop for this path's sake)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rx[i % 2] = rb[i] = u32x4{0, 0, 0, 0};
+            rl = rt = rd = 0.0f;
+        }
         bf16* slot = slots + (size_t)c * (2 * FN * FP);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -547,24 +574,31 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     auto fetch = [&](uint32_t v) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
         const size_t row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
+        // rows behind the sequence's end are out of the resource's range: zeros
+        const uint32_t range = (uint32_t)(((tl - 1) * hp + FP) * sizeof(bf16));
+        const auto xr = rsrc((const bf16*)a.X + row0, range), yr = rsrc((const bf16*)a.dY + row0, range);
+        const uint32_t step = (uint32_t)hp * (F_NT / (FP / 8) * sizeof(bf16));
+        const uint32_t at = (tid / (FP / 8)) * (uint32_t)(hp * sizeof(bf16)) + tid % (FP / 8) * 16;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            rx[i] = piece((const bf16*)a.X + row0, hp, tl, FP / 8, tid + i * F_NT);
-            ry[i] = piece((const bf16*)a.dY + row0, hp, tl, FP / 8, tid + i * F_NT);
+            rx[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, at, i * step, 0);
+            ry[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, at, i * step, 0);
         }
         const size_t slot = ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * (2 * FN * FP);
-        const bf16 *gs = (const bf16*)a.gst + slot, *hs = (const bf16*)a.hst + slot;
+        const auto gr = rsrc((const bf16*)a.gst + slot, 2 * FN * FP * 2), hr = rsrc((const bf16*)a.hst + slot, 2 * FN * FP * 2);
+        const uint32_t ha = ((16 * w + li) * FP + 8 * lq) * 2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            rg[i] = *reinterpret_cast<const u32x4*>(gs + 8 * (size_t)(tid + i * F_NT));
-            rh[i] = *reinterpret_cast<const u32x4*>(hs + (i / 2) * (FN * FP) + (16 * w + li) * FP + 32 * (i % 2) + 8 * lq);
+            rg[i] = __builtin_amdgcn_raw_buffer_load_b128(gr, 16 * tid, i * F_NT * 16, 0);
+            rh[i] = __builtin_amdgcn_raw_buffer_load_b128(hr, ha, (i / 2) * (FN * FP * 2) + (i % 2) * 64, 0);
         }
-        const float* lc = a.lc + (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
-        const uint32_t t = tid % FQ;
-        rl = lc[t];
+        const size_t sp0 = (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
+        const float *lc = a.lc + sp0, *dv = a.dtv + sp0;
+        const uint32_t tt = tid % FQ;
+        rl = lc[tt];
         rt = lc[FQ - 1];
-        rr = t >= 16 ? lc[t / 16 * 16 - 1] : 0.0f;
-        rd = a.dtv[(((size_t)b * a.H + h) * a.nchunk + c) * FQ + t];
+        rr = lc[tt >= 16 ? tt / 16 * 16 - 1 : 0];      // (token blocks past the first)
+        rd = dv[tt];
     };
 
     // C B^T, lower tiles
@@ -763,7 +797,16 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 }
             }
         }
-        if (v + 1 < v_end) fetch(v + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (v + 1 < v_end) {
+            fetch(v + 1);
+        } else {
+            // (not kept over the loop for this path's sake)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rx[i % 2] = ry[i % 2] = rg[i] = rh[i] = u32x4{0, 0, 0, 0};
+            rl = rt = rr = rd = 0.0f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
         col = swap_add32(swap_add16(col));
         if (lq == 0) {
             UO[j] = uo;
@@ -775,20 +818,21 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             red[w][1] = diag;
         }
         const float D = a.D ? to_f(((const bf16*)a.D)[h]) : 0.0f;
-        bf16* out = (bf16*)a.dX + ((size_t)b * L + t0 + j) * hp + (size_t)h * P + sl * FP;
+        bf16* out0 = (bf16*)a.dX + ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
+        const uint32_t out = j * (uint32_t)hp + 4 * lq;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             const s4v y = *reinterpret_cast<const s4v*>(Ys + j * FXP + 16 * p + 4 * lq);
             floatx4 o;
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = fmaf(dtj, dx[p][r], D * val(y[r]));
-            if (j < (int)tl) *reinterpret_cast<s4v*>(out + 16 * p + 4 * lq) = take4(o);
+            if (j < (int)tl) *reinterpret_cast<s4v*>(out0 + (out + 16 * p)) = take4(o);
         }
         lds_barrier();
         // a_t: pairs of a source before t and a sink from t on; lane l has
         // tokens 2 l and 2 l + 1
         if (w == 7) {
-            float pre[2], suf[2], dir[2], dt[2];
+            float pre[2], suf[2], dir[2], dt[2], slope[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int t = 2 * lane + k;
@@ -797,6 +841,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 for (int i = 0; i < 8; ++i) s += VO[i][t];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s += RS[i][t];
+                slope[k] = a.slope[(((size_t)b * a.H + h) * a.nchunk + c) * FQ + t];
                 dt[k] = DT[t];
                 dir[k] = UO[t] + CS[t];
                 pre[k] = dt[k] * UO[t];
@@ -812,18 +857,20 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 dd += red[i][1];
             }
             const float edge = __expf(LC[FQ - 1]) * e0, A = -expf(to_f(((const bf16*)a.A_log)[h]));
-            float da[2];
+            float da[2], q[2];
             da[0] = edge + p_in + (s_from + own);
             da[1] = edge + (p_in + pre[0]) + (s_from + suf[1]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (2 * lane + k < (int)tl)
-                    a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + 2 * lane + k] = dir[k] + A * da[k];
-            const float dA = wave_sum(dt[0] * da[0] + dt[1] * da[1]);
+            for (int k = 0; k < 2; ++k) {
+                q[k] = (dir[k] + A * da[k]) * slope[k];
+                if (2 * lane + k < (int)tl) a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + 2 * lane + k] = q[k];
+            }
+            const float dA = wave_sum(dt[0] * da[0] + dt[1] * da[1]), dq = wave_sum(q[0] + q[1]);
             if (lane == 0) {
-                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 2;
-                o[0] = A * dA;
-                o[1] = dd;
+                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 3;
+                o[0] = dq;
+                o[1] = A * dA;
+                o[2] = dd;
             }
         }
     }
@@ -880,7 +927,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         for (int r = 0; r < 4; ++r) {
             const uint32_t t = 16 * T + 4 * lq + r;
             if (t < tl) {
-                const size_t at = ((((size_t)sp * a.batch + b) * L + t0 + t) * a.G + g) * FN + 16 * w + li;
+                const size_t at = (size_t)sp * a.share + (((size_t)b * L + t0 + t) * a.G + g) * FN + 16 * w + li;
                 a.cpart[at] = dc[T][r];
                 a.bpart[at] = db[T][r];
             }
@@ -891,63 +938,79 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
 // ---------------------------------------------------------------------------
 // Sums over shares, slices and chunks
 // ---------------------------------------------------------------------------
-// gradient of raw + bias from that of dt: the softplus' slope, 0 where the
-// clamp holds
-template <typename T> __device__ __forceinline__ float dt_slope(const SsdBwdArgs& a, uint32_t b, uint32_t t, uint32_t h) {
-    const float v = to_f(((const T*)a.dt)[((size_t)b * a.L + t) * a.H + h]) + to_f(((const T*)a.dt_bias)[h]);
-    const float sp = v > 20.0f ? v : log1pf(expf(v));
-    return sp >= a.dt_min && sp <= a.dt_max ? 1.0f / (1.0f + expf(-v)) : 0.0f;
-}
-__device__ __forceinline__ float dt_grad(const SsdBwdArgs& a, uint32_t b, uint32_t t, uint32_t h) {
-    float s = 0.0f;
-    for (uint32_t i = 0; i < a.nslice; ++i) s += a.q[(((size_t)i * a.batch + b) * a.H + h) * a.L + t];
-    return s;
+// One launch: blocks of four dB and dC elements a thread, then blocks of 64
+// tokens by 16 heads of d_dt (which the chunks left a head at a time), then a
+// block a head for the parameters' gradients, summed in 64 bits.
+constexpr int R_NT = 256, R_T = 64, R_H = 16;
+
+template <typename T> __device__ __forceinline__ void store4(T* dst, size_t i, size_t n, const float (&v)[4]) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (i + 4 <= n && (uintptr_t)dst % sizeof(T4) == 0) {
+        *reinterpret_cast<T4*>(dst + i) = T4{from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};
+    } else {
+        for (int e = 0; e < 4 && i + e < n; ++e) dst[i + e] = from_f<T>(v[e]);
+    }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void ssd_bwd_rows_kernel(SsdBwdArgs a) {
-    const size_t nb = (size_t)a.batch * a.L * a.G * a.N, nt = (size_t)a.batch * a.L * a.H;
-    const size_t step = (size_t)gridDim.x * 256;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < nb; i += step) {
-        float x = 0.0f, y = 0.0f;
+template <typename T> __global__ __launch_bounds__(R_NT) void ssd_bwd_finish_kernel(SsdBwdArgs a) {
+    __shared__ union {
+        float tile[R_T][R_H + 1];
+        double red[3][R_NT];
+    } sh;
+    const uint32_t tid = threadIdx.x;
+    uint32_t blk = blockIdx.x;
+    if (blk < a.row_blocks) {
+        const size_t n = (size_t)a.batch * a.L * a.G * a.N, i = ((size_t)blk * R_NT + tid) * 4;
+        if (i >= n) return;
+        float x[4] = {}, y[4] = {};
         for (uint32_t s = 0; s < a.nsplit; ++s) {
-            x += a.bpart[s * nb + i];
-            y += a.cpart[s * nb + i];
+            const floatx4 u = *reinterpret_cast<const floatx4*>(a.bpart + s * a.share + i);
+            const floatx4 v = *reinterpret_cast<const floatx4*>(a.cpart + s * a.share + i);
+            for (int e = 0; e < 4; ++e) {
+                x[e] += u[e];
+                y[e] += v[e];
+            }
         }
-        ((T*)a.dB)[i] = from_f<T>(x);
-        ((T*)a.dC)[i] = from_f<T>(y);
+        store4((T*)a.dB, i, n, x);
+        store4((T*)a.dC, i, n, y);
+        return;
     }
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < nt; i += step) {
-        const uint32_t h = i % a.H, b = i / a.H / a.L, t = i / a.H % a.L;
-        ((T*)a.d_dt)[i] = from_f<T>(dt_grad(a, b, t, h) * dt_slope<T>(a, b, t, h));
+    blk -= a.row_blocks;
+    if (blk < a.dt_blocks) {
+        const uint32_t nh = (a.H + R_H - 1) / R_H, nt = (a.L + R_T - 1) / R_T;
+        const uint32_t h0 = blk % nh * R_H, t0 = blk / nh % nt * R_T, b = blk / nh / nt;
+        for (uint32_t i = tid; i < R_T * R_H; i += R_NT) {
+            const uint32_t h = i / R_T, t = i % R_T;
+            if (h0 + h >= a.H || t0 + t >= a.L) continue;
+            float v = 0.0f;
+            for (uint32_t s = 0; s < a.nslice; ++s) v += a.q[(((size_t)s * a.batch + b) * a.H + h0 + h) * a.L + t0 + t];
+            sh.tile[t][h] = v;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < R_T * R_H; i += R_NT) {
+            const uint32_t t = i / R_H, h = i % R_H;
+            if (h0 + h < a.H && t0 + t < a.L) ((T*)a.d_dt)[((size_t)b * a.L + t0 + t) * a.H + h0 + h] = from_f<T>(sh.tile[t][h]);
+        }
+        return;
     }
-}
-
-// A head's sums over all tokens, in 64 bits: a block a head.
-template <typename T> __global__ __launch_bounds__(256) void ssd_bwd_heads_kernel(SsdBwdArgs a) {
-    __shared__ double red[3][256];
-    const uint32_t h = blockIdx.x, tid = threadIdx.x;
+    const uint32_t h = blk - a.dt_blocks;
     double s[3] = {0, 0, 0};
-    for (size_t i = tid; i < (size_t)a.batch * a.L; i += 256) {
-        const uint32_t b = i / a.L, t = i % a.L;
-        s[0] += (double)(dt_grad(a, b, t, h) * dt_slope<T>(a, b, t, h));
-    }
     const size_t np = (size_t)a.nslice * a.nchunk;
-    for (size_t i = tid; i < a.batch * np; i += 256) {
-        const float* o = a.part + (((size_t)(i / np) * a.H + h) * np + i % np) * 2;
-        s[1] += (double)o[0];
-        s[2] += (double)o[1];
+    for (size_t i = tid; i < a.batch * np; i += R_NT) {
+        const float* o = a.part + (((size_t)(i / np) * a.H + h) * np + i % np) * 3;
+        for (int k = 0; k < 3; ++k) s[k] += (double)o[k];
     }
-    for (int k = 0; k < 3; ++k) red[k][tid] = s[k];
+    for (int k = 0; k < 3; ++k) sh.red[k][tid] = s[k];
     __syncthreads();
-    for (int d = 128; d; d >>= 1) {
+    for (int d = R_NT / 2; d; d >>= 1) {
         if ((int)tid < d)
-            for (int k = 0; k < 3; ++k) red[k][tid] += red[k][tid + d];
+            for (int k = 0; k < 3; ++k) sh.red[k][tid] += sh.red[k][tid + d];
         __syncthreads();
     }
     if (tid == 0) {
-        ((T*)a.d_dt_bias)[h] = from_f<T>((float)red[0][0]);
-        ((T*)a.dA_log)[h] = from_f<T>((float)red[1][0]);
-        if (a.dD) ((T*)a.dD)[h] = from_f<T>((float)red[2][0]);
+        ((T*)a.d_dt_bias)[h] = from_f<T>((float)sh.red[0][0]);
+        ((T*)a.dA_log)[h] = from_f<T>((float)sh.red[1][0]);
+        if (a.dD) ((T*)a.dD)[h] = from_f<T>((float)sh.red[2][0]);
     }
 }
 
@@ -957,12 +1020,12 @@ template <typename F> hipError_t with_type(int act, F f) {
     return f(float{});
 }
 
-// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts][steps]
+// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts][3 x steps]
 struct Plan {
     bool fast;
     uint32_t nchunk, nslice, nsplit;
-    size_t states, rows, q, part, steps;      // floats of one of each
-    size_t floats() const { return 2 * states + 2 * rows + q + part + 2 * steps; }
+    size_t states, share, q, part, steps;      // floats of one of each
+    size_t floats() const { return 2 * states + 2 * nsplit * share + q + part + 3 * steps; }
 };
 Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     Plan p;
@@ -985,15 +1048,18 @@ Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
         }
     }
     p.states = (size_t)batch * d.H * p.nchunk * d.P * d.N;
-    p.rows = (size_t)p.nsplit * batch * d.L * d.n_groups * d.N;
+    p.share = (size_t)batch * d.L * d.n_groups * d.N;
     p.q = (size_t)p.nslice * batch * d.H * d.L;
-    p.part = (size_t)batch * d.H * p.nslice * p.nchunk * 2;
+    p.part = (size_t)batch * d.H * p.nslice * p.nchunk * 3;
     p.steps = fast ? (size_t)batch * d.H * p.nchunk * FQ : 0;
     // every array starts on a 16-byte address
-    for (size_t* n : {&p.states, &p.rows, &p.q, &p.part, &p.steps}) *n = (*n + 3) / 4 * 4;
+    for (size_t* n : {&p.states, &p.share, &p.q, &p.part, &p.steps}) *n = (*n + 3) / 4 * 4;
     return p;
 }
-bool fast_dims(const lssm_ssd_dims& d, int act) { return act == LSSM_BF16 && d.N == FN && d.P % FP == 0; }
+// (a chunk's rows within 32-bit byte offsets)
+bool fast_dims(const lssm_ssd_dims& d, int act) {
+    return act == LSSM_BF16 && d.N == FN && d.P % FP == 0 && (uint64_t)d.H * d.P * FQ * 2 < (1u << 31);
+}
 
 template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArgs& a) {
     ssd_bwd_walk_kernel<T, NT><<<dim3(a.H * a.nslice, a.batch, 2), G_NT, 0, s>>>(a);
@@ -1020,11 +1086,15 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
     a.hst = static_cast<float*>(ws);
     a.gst = a.hst + p.states;
     a.bpart = a.gst + p.states;
-    a.cpart = a.bpart + p.rows;
-    a.q = a.cpart + p.rows;
+    a.cpart = a.bpart + p.nsplit * p.share;
+    a.q = a.cpart + p.nsplit * p.share;
     a.part = a.q + p.q;
     a.lc = a.part + p.part;
     a.dtv = a.lc + p.steps;
+    a.slope = a.dtv + p.steps;
+    a.share = p.share;
+    a.row_blocks = (uint32_t)((p.share + 4 * R_NT - 1) / (4 * R_NT));
+    a.dt_blocks = a.batch * ((a.L + R_T - 1) / R_T) * ((a.H + R_H - 1) / R_H);
     return with_type(act, [&](auto z) {
         using T = decltype(z);
         if (a.batch) {
@@ -1036,11 +1106,8 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
             } else if (a.N <= 64) launch_generic<T, 64>(s, a);
             else if (a.N <= 128) launch_generic<T, 128>(s, a);
             else launch_generic<T, 256>(s, a);
-            const size_t n = (size_t)a.batch * a.L * std::max(a.G * a.N, a.H);
-            if (n)
-                ssd_bwd_rows_kernel<T><<<(uint32_t)std::min<size_t>((n + 255) / 256, 4096), 256, 0, s>>>(a);
         }
-        ssd_bwd_heads_kernel<T><<<a.H, 256, 0, s>>>(a);
+        ssd_bwd_finish_kernel<T><<<a.row_blocks + a.dt_blocks + a.H, R_NT, 0, s>>>(a);
         return hipGetLastError();
     });
 }
