@@ -29,6 +29,7 @@
 // heads, slices and chunks.  Every order of summation is fixed.
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -426,85 +427,98 @@ __device__ __forceinline__ u32x4 piece(const bf16* src, size_t stride, uint32_t 
     return r < rows ? *reinterpret_cast<const u32x4*>(src + r * stride + 8 * c) : u32x4{0, 0, 0, 0};
 }
 
-// The walk: block (head, slice), sequence, direction; wave (pt, nh) keeps the
-// state's rows 16 pt .. + 15 and columns 64 nh .. + 63 in fp32.  A chunk's
-// state goes out as two pieces, [piece][n][row], the order in which the
-// chunks' kernel takes it as an operand.
-__global__ __launch_bounds__(F_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
-    __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * FBP];
+// where tile (row tile, column tile) of a kept state's piece starts
+__device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt, uint32_t piece) {
+    return ((pt * (FN / 16) + nt) * 2 + piece) * 256;
+}
+
+// The walk: block (head, slice, part of the state's columns), sequence,
+// direction; wave w keeps the state's rows 16 w .. + 15, all NC columns of the
+// part, in fp32.  A chunk's state goes out as two pieces, in tiles of 16 rows by
+// 16 columns ([row tile][column tile][piece][n][row]): what a wave stores at
+// once is contiguous (32 bytes of each of four waves to a line stored at 3.0
+// TB/s), and a lane of the chunks' kernel finds its operand in 16 bytes.
+constexpr int W_NT = 256;
+template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
+    constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 8;
+    constexpr int XV = FQ * FP / 8 / W_NT, BV = FQ * NC / 8 / W_NT;     // 16-byte pieces a thread stages
+    __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * BP];
     __shared__ __attribute__((aligned(16))) float W[FQ];
-    __shared__ float Dq;
-    const uint32_t h = blockIdx.x / a.nslice, sl = blockIdx.x % a.nslice, b = blockIdx.y;
+    const uint32_t n0 = blockIdx.x % PARTS * NC, h = blockIdx.x / PARTS / a.nslice, sl = blockIdx.x / PARTS % a.nslice;
+    const uint32_t b = blockIdx.y;
     const bool back = blockIdx.z != 0;
     const uint32_t P = a.P, L = a.L, g = h / (a.H / a.G), tid = threadIdx.x;
     const int lane = tid % WAVE, li = lane % 16, lq = lane / 16, tk = li / 4, tc = li % 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE), pt = w % 4, nh = w / 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const float* init = back ? a.d_state : a.state;
     bf16* slots = (bf16*)(back ? a.gst : a.hst) + (((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk * (2 * FN * FP);
     const bf16* rows = (const bf16*)(back ? a.dY : a.X) + (size_t)b * L * a.H * P + (size_t)h * P + sl * FP;
-    const bf16* cols = (const bf16*)(back ? a.C : a.B) + (size_t)b * L * a.G * FN + (size_t)g * FN;
+    const bf16* cols = (const bf16*)(back ? a.C : a.B) + (size_t)b * L * a.G * FN + (size_t)g * FN + n0;
     const float* lc = a.lc + ((size_t)b * a.H + h) * a.nchunk * FQ;
     const float* dtv = a.dtv + ((size_t)b * a.H + h) * a.nchunk * FQ;
-    const size_t plain = (((size_t)b * a.H + h) * P + sl * FP + 16 * pt + 4 * lq) * FN + 64 * nh + li;
+    const size_t plain = (((size_t)b * a.H + h) * P + sl * FP + 16 * w + 4 * lq) * FN + n0 + li;
 
-    floatx4 s[4];
+    floatx4 s[NTL];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NTL; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[i][r] = init ? init[plain + r * FN + 16 * i] : 0.0f;
 
-    u32x4 rx[2], rb[4];
+    u32x4 rx[XV], rb[BV];
     float rl = 0.0f, rt = 0.0f, rd = 0.0f;
-    auto fetch = [&](uint32_t c) {
+    // the chunk's rows (behind the sequence's end, and for live = false: zeros,
+    // as out of the resource's range)
+    const uint32_t xat = tid / (FP / 8) * (a.H * P * 2) + tid % (FP / 8) * 16;
+    const uint32_t bat = tid / (NC / 8) * (a.G * FN * 2) + tid % (NC / 8) * 16;
+    auto fetch = [&](uint32_t c, bool live) {
         const uint32_t t0 = c * FQ, tl = min((uint32_t)FQ, L - t0);
+        const auto xr = rsrc(rows + (size_t)t0 * a.H * P, live ? ((tl - 1) * a.H * P + FP) * 2 : 0);
+        const auto br = rsrc(cols + (size_t)t0 * a.G * FN, live ? ((tl - 1) * a.G * FN + NC) * 2 : 0);
+        const auto lr = rsrc(lc + t0, live ? FQ * 4 : 0), dr = rsrc(dtv + t0, live ? FQ * 4 : 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) rx[i] = piece(rows + (size_t)t0 * a.H * P, (size_t)a.H * P, tl, FP / 8, tid + i * F_NT);
+        for (int i = 0; i < XV; ++i)
+            rx[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, xat, i * (W_NT / (FP / 8)) * a.H * P * 2, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rb[i] = piece(cols + (size_t)t0 * a.G * FN, (size_t)a.G * FN, tl, FN / 8, tid + i * F_NT);
-        rl = lc[t0 + tid % FQ];
-        rt = lc[t0 + FQ - 1];
-        rd = dtv[t0 + tid % FQ];
+        for (int i = 0; i < BV; ++i)
+            rb[i] = __builtin_amdgcn_raw_buffer_load_b128(br, bat, i * (W_NT / (NC / 8)) * a.G * FN * 2, 0);
+        rl = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, tid % FQ * 4, 0, 0));
+        rt = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (FQ - 1) * 4, 0, 0));
+        rd = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(dr, tid % FQ * 4, 0, 0));
     };
-    const uint32_t first = back ? a.nchunk - 1 : 0;
-    if (a.nchunk) fetch(first);
+    if (a.nchunk) fetch(back ? a.nchunk - 1 : 0, true);
     for (uint32_t k = 0; k < a.nchunk; ++k) {
         const uint32_t c = back ? a.nchunk - 1 - k : k;
         lds_barrier();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t j = tid + i * F_NT;
+        for (int i = 0; i < XV; ++i) {
+            const uint32_t j = tid + i * W_NT;
             *reinterpret_cast<u32x4*>(Xs + j / (FP / 8) * FXP + j % (FP / 8) * 8) = rx[i];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t j = tid + i * F_NT;
-            *reinterpret_cast<u32x4*>(Bs + j / (FN / 8) * FBP + j % (FN / 8) * 8) = rb[i];
+        for (int i = 0; i < BV; ++i) {
+            const uint32_t j = tid + i * W_NT;
+            *reinterpret_cast<u32x4*>(Bs + j / (NC / 8) * BP + j % (NC / 8) * 8) = rb[i];
         }
-        if (tid < FQ) W[tid] = back ? __expf(rl) : rd * __expf(rt - rl);
-        if (tid == 0) Dq = __expf(rt);
+        W[tid % FQ] = (back ? 1.0f : rd) * __expf(back ? rl : rt - rl);      // (both halves of the block the same)
+        const float dq = __expf(rt);
         lds_barrier();
-        if (k + 1 < a.nchunk) {
-            fetch(back ? c - 1 : c + 1);
-        } else {
-            // (not kept over the loop for this path's sake)
+        bf16* slot = slots + (size_t)c * (2 * FN * FP) + state_at(w, n0 / 16, 0) + 16 * li + 4 * lq;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rx[i % 2] = rb[i] = u32x4{0, 0, 0, 0};
-            rl = rt = rd = 0.0f;
-        }
-        bf16* slot = slots + (size_t)c * (2 * FN * FP);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bf16* o = slot + (64 * nh + 16 * i + li) * FP + 16 * pt + 4 * lq;
+        for (int i = 0; i < NTL; ++i) {
             floatx4 v = s[i];
-            *reinterpret_cast<s4v*>(o) = take4(v);
-            *reinterpret_cast<s4v*>(o + FN * FP) = take4(v);
+            *reinterpret_cast<s4v*>(slot + state_at(0, i, 0)) = take4(v);
+            *reinterpret_cast<s4v*>(slot + state_at(0, i, 1)) = take4(v);
+            s[i] *= dq;
         }
-        const float dq = Dq;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] *= dq;
+        // the next chunk's loads are the youngest accesses: waiting for them
+        // at the top waits for nothing that was issued later
+        fetch(back ? max(c, 1u) - 1 : min(c + 1, a.nchunk - 1), k + 1 < a.nchunk);
+        // the weighted rows in three pieces: the gradient of the first state is
+        // given in fp32
+        s8v f[FQ / 32][3];
 #pragma unroll
         for (int ks = 0; ks < FQ / 32; ++ks) {
-            const bf16* xp = Xs + (32 * ks + 8 * lq + tk) * FXP + 16 * pt + 4 * tc;
+            const bf16* xp = Xs + (32 * ks + 8 * lq + tk) * FXP + 16 * w + 4 * tc;
             const s4v x0 = ld_tr(xp), x1 = ld_tr(xp + 4 * FXP);
             floatx4 v0 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq);
             floatx4 v1 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq + 4);
@@ -513,25 +527,25 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
                 v0[e] *= val(x0[e]);
                 v1[e] *= val(x1[e]);
             }
-            // three pieces: the gradient of the first state is given in fp32
-            s8v f[3];
 #pragma unroll
             for (int e = 0; e < 3; ++e) {
                 const s4v lo = take4(v0);
-                f[e] = cat8(lo, take4(v1));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bf16* bp = Bs + (32 * ks + 8 * lq + tk) * FBP + 64 * nh + 16 * i + 4 * tc;
-                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 4 * FBP));
-#pragma unroll
-                for (int e = 0; e < 3; ++e) s[i] = mma(f[e], bt, s[i]);
+                f[ks][e] = cat8(lo, take4(v1));
             }
         }
+#pragma unroll
+        for (int ks = 0; ks < FQ / 32; ++ks)
+#pragma unroll
+            for (int i = 0; i < NTL; ++i) {
+                const bf16* bp = Bs + (32 * ks + 8 * lq + tk) * BP + 16 * i + 4 * tc;
+                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 4 * BP));
+#pragma unroll
+                for (int e = 0; e < 3; ++e) s[i] = mma(f[ks][e], bt, s[i]);
+            }
     }
     if (back && a.d_state0)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NTL; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) a.d_state0[plain + r * FN + 16 * i] = s[i][r];
 }
@@ -571,11 +585,11 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     const uint32_t v_first = sp * per, v_end = min(pairs, v_first + per);
     u32x4 rx[2], ry[2], rg[4], rh[4];
     float rl = 0.0f, rt = 0.0f, rr = 0.0f, rd = 0.0f;
-    auto fetch = [&](uint32_t v) {
+    auto fetch = [&](uint32_t v, bool live) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
         const size_t row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
         // rows behind the sequence's end are out of the resource's range: zeros
-        const uint32_t range = (uint32_t)(((tl - 1) * hp + FP) * sizeof(bf16));
+        const uint32_t range = live ? (uint32_t)(((tl - 1) * hp + FP) * sizeof(bf16)) : 0u, whole = live ? 2 * FN * FP * 2 : 0;
         const auto xr = rsrc((const bf16*)a.X + row0, range), yr = rsrc((const bf16*)a.dY + row0, range);
         const uint32_t step = (uint32_t)hp * (F_NT / (FP / 8) * sizeof(bf16));
         const uint32_t at = (tid / (FP / 8)) * (uint32_t)(hp * sizeof(bf16)) + tid % (FP / 8) * 16;
@@ -585,20 +599,21 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             ry[i] = __builtin_amdgcn_raw_buffer_load_b128(yr, at, i * step, 0);
         }
         const size_t slot = ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * (2 * FN * FP);
-        const auto gr = rsrc((const bf16*)a.gst + slot, 2 * FN * FP * 2), hr = rsrc((const bf16*)a.hst + slot, 2 * FN * FP * 2);
-        const uint32_t ha = ((16 * w + li) * FP + 8 * lq) * 2;
+        const auto gr = rsrc((const bf16*)a.gst + slot, whole), hr = rsrc((const bf16*)a.hst + slot, whole);
+        const uint32_t ha = (state_at(lq / 2, w, 0) + 16 * li + 8 * (lq % 2)) * 2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             rg[i] = __builtin_amdgcn_raw_buffer_load_b128(gr, 16 * tid, i * F_NT * 16, 0);
-            rh[i] = __builtin_amdgcn_raw_buffer_load_b128(hr, ha, (i / 2) * (FN * FP * 2) + (i % 2) * 64, 0);
+            rh[i] = __builtin_amdgcn_raw_buffer_load_b128(hr, ha, state_at(2 * (i % 2), 0, i / 2) * 2, 0);
         }
         const size_t sp0 = (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
-        const float *lc = a.lc + sp0, *dv = a.dtv + sp0;
+        const auto lr = rsrc(a.lc + sp0, live ? FQ * 4 : 0), dr = rsrc(a.dtv + sp0, live ? FQ * 4 : 0);
         const uint32_t tt = tid % FQ;
-        rl = lc[tt];
-        rt = lc[FQ - 1];
-        rr = lc[tt >= 16 ? tt / 16 * 16 - 1 : 0];      // (token blocks past the first)
-        rd = dv[tt];
+        auto one = [](auto r, uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * at, 0, 0)); };
+        rl = one(lr, tt);
+        rt = one(lr, FQ - 1);
+        rr = one(lr, tt >= 16 ? tt / 16 * 16 - 1 : 0);      // (token blocks past the first)
+        rd = one(dr, tt);
     };
 
     // C B^T, lower tiles
@@ -638,7 +653,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     floatx4 dc[8], db[8];
 #pragma unroll
     for (int T = 0; T < 8; ++T) dc[T] = db[T] = floatx4{0, 0, 0, 0};
-    if (v_first < v_end) fetch(v_first);
+    if (v_first < v_end) fetch(v_first, true);
 
     for (uint32_t v = v_first; v < v_end; ++v) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
@@ -656,8 +671,9 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t j = (tid + i * F_NT) % (FN * FP / 8);
-            *reinterpret_cast<u32x4*>((i < 2 ? Gh : Gl) + j / (FP / 8) * FXP + j % (FP / 8) * 8) = rg[i];
+            // 16 bytes j of the state: 32 a tile's piece
+            const uint32_t j = tid + i * F_NT, pc = j / 32 % 2, nt = j / 64 % (FN / 16), pt = j / 64 / (FN / 16);
+            *reinterpret_cast<u32x4*>((pc ? Gl : Gh) + (16 * nt + j % 32 / 2) * FXP + 16 * pt + 8 * (j % 2)) = rg[i];
         }
         if (tid < FQ) {
             const float er = __expf(rt - rl);
@@ -797,16 +813,6 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 }
             }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (v + 1 < v_end) {
-            fetch(v + 1);
-        } else {
-            // (not kept over the loop for this path's sake)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rx[i % 2] = ry[i % 2] = rg[i] = rh[i] = u32x4{0, 0, 0, 0};
-            rl = rt = rr = rd = 0.0f;
-        }
-        __builtin_amdgcn_sched_barrier(0);
         col = swap_add32(swap_add16(col));
         if (lq == 0) {
             UO[j] = uo;
@@ -828,6 +834,9 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             for (int r = 0; r < 4; ++r) o[r] = fmaf(dtj, dx[p][r], D * val(y[r]));
             if (j < (int)tl) *reinterpret_cast<s4v*>(out0 + (out + 16 * p)) = take4(o);
         }
+        // behind the stores: waiting for the next pair at the top waits for
+        // nothing that was issued later
+        fetch(min(v + 1, v_end - 1), v + 1 < v_end);
         lds_barrier();
         // a_t: pairs of a source before t and a sink from t on; lane l has
         // tokens 2 l and 2 l + 1
@@ -1100,7 +1109,11 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
         if (a.batch) {
             if (fast) {
                 if (a.nchunk) ssd_bwd_steps_kernel<<<dim3(a.nchunk, a.H, a.batch), FQ, 0, s>>>(a);
-                ssd_bwd_walk_bf16_kernel<<<dim3(a.H * a.nslice, a.batch, 2), F_NT, 0, s>>>(a);
+                const char* ev = getenv("WALK_NC");
+                const int nc = ev ? atoi(ev) : 128;
+                if (nc == 128) ssd_bwd_walk_bf16_kernel<128><<<dim3(a.H * a.nslice, a.batch, 2), W_NT, 0, s>>>(a);
+                else if (nc == 64) ssd_bwd_walk_bf16_kernel<64><<<dim3(a.H * a.nslice * 2, a.batch, 2), W_NT, 0, s>>>(a);
+                else ssd_bwd_walk_bf16_kernel<32><<<dim3(a.H * a.nslice * 4, a.batch, 2), W_NT, 0, s>>>(a);
                 if (a.nchunk)
                     ssd_bwd_chunk_bf16_kernel<<<dim3(a.nchunk * a.nsplit * a.G, a.batch), F_NT, 0, s>>>(a);
             } else if (a.N <= 64) launch_generic<T, 64>(s, a);
