@@ -354,7 +354,7 @@ constexpr int FQ = 128;      // tokens a chunk
 constexpr int FP = 64;       // state rows a slice
 constexpr int FN = 128;      // state size
 constexpr int FXP = FP + 8;  // pitch of a [token or n][row] tile
-constexpr int FBP = FN + 8;  // pitch of a [token][n] tile
+constexpr int FBP = FN + 16; // pitch of a [token][n] tile
 constexpr int F_NT = 512;
 
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -440,7 +440,7 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // TB/s), and a lane of the chunks' kernel finds its operand in 16 bytes.
 constexpr int W_NT = 256;
 template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
-    constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 8;
+    constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 16;
     constexpr int XV = FQ * FP / 8 / W_NT, BV = FQ * NC / 8 / W_NT;     // 16-byte pieces a thread stages
     __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * BP];
     __shared__ __attribute__((aligned(16))) float W[FQ];
@@ -518,10 +518,12 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
         s8v f[FQ / 32][3];
 #pragma unroll
         for (int ks = 0; ks < FQ / 32; ++ks) {
-            const bf16* xp = Xs + (32 * ks + 8 * lq + tk) * FXP + 16 * w + 4 * tc;
-            const s4v x0 = ld_tr(xp), x1 = ld_tr(xp + 4 * FXP);
-            floatx4 v0 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq);
-            floatx4 v1 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 8 * lq + 4);
+            // k = token in the order 4 q .. + 3, 16 + 4 q .. + 3 of each 32:
+            // the transposing loads meet no bank twice
+            const bf16* xp = Xs + (32 * ks + 4 * lq + tk) * FXP + 16 * w + 4 * tc;
+            const s4v x0 = ld_tr(xp), x1 = ld_tr(xp + 16 * FXP);
+            floatx4 v0 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 4 * lq);
+            floatx4 v1 = *reinterpret_cast<const floatx4*>(W + 32 * ks + 16 + 4 * lq);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v0[e] *= val(x0[e]);
@@ -537,8 +539,8 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
         for (int ks = 0; ks < FQ / 32; ++ks)
 #pragma unroll
             for (int i = 0; i < NTL; ++i) {
-                const bf16* bp = Bs + (32 * ks + 8 * lq + tk) * BP + 16 * i + 4 * tc;
-                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 4 * BP));
+                const bf16* bp = Bs + (32 * ks + 4 * lq + tk) * BP + 16 * i + 4 * tc;
+                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 16 * BP));
 #pragma unroll
                 for (int e = 0; e < 3; ++e) s[i] = mma(f[ks][e], bt, s[i]);
             }
@@ -563,11 +565,23 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
 constexpr int F_TILES = 36;
 __device__ __forceinline__ constexpr int tile_of(int T, int J) { return T * (T + 1) / 2 + J; }
 
+// Sums over the 16 lanes of a row of four values each; lane i ends with that
+// of value i % 4.
+__device__ __forceinline__ float row_sums4(const floatx4& v) {
+    const uint32_t l = threadIdx.x;
+    const bool b0 = l & 1, b1 = l & 2;
+    const float a = (b0 ? v[1] : v[0]) + dpp_f32<0xB1>(b0 ? v[0] : v[1]);      // values 0, 1
+    const float c = (b0 ? v[3] : v[2]) + dpp_f32<0xB1>(b0 ? v[2] : v[3]);      // values 2, 3
+    float s = (b1 ? c : a) + dpp_f32<0x4E>(b1 ? a : c);
+    s += dpp_f32<0x124>(s);                                                    // row_ror:4
+    return s + dpp_f32<0x128>(s);                                              // row_ror:8
+}
+
 __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) {
     __shared__ __attribute__((aligned(16))) bf16 stage[4 * FQ * FXP];
     __shared__ __attribute__((aligned(16))) floatx4 SS[F_TILES * WAVE], CB[F_TILES * WAVE];
     __shared__ __attribute__((aligned(16))) float LC[FQ], DT[FQ], EL[FQ], ER[FQ], WB[FQ], AF[FQ];
-    __shared__ float VO[8][FQ], RS[8][FQ], UO[FQ], CS[FQ], red[8][2];
+    __shared__ float SL[FQ], VO[8][FQ], RS[8][FQ], UO[FQ], CS[FQ], red[8][2];
     bf16 *Xs = stage, *Ys = stage + FQ * FXP, *Gh = stage + 2 * FQ * FXP, *Gl = stage + 3 * FQ * FXP;
     const uint32_t P = a.P, L = a.L, hpg = a.H / a.G;
     uint32_t tid = threadIdx.x;
@@ -584,7 +598,8 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     const uint32_t pairs = hpg * a.nslice, per = (pairs + a.nsplit - 1) / a.nsplit;
     const uint32_t v_first = sp * per, v_end = min(pairs, v_first + per);
     u32x4 rx[2], ry[2], rg[4], rh[4];
-    float rl = 0.0f, rt = 0.0f, rr = 0.0f, rd = 0.0f;
+    float rl = 0.0f, rt = 0.0f, rr = 0.0f, rd = 0.0f, rs = 0.0f;
+    uint32_t ra = 0, rD = 0;
     auto fetch = [&](uint32_t v, bool live) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
         const size_t row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
@@ -607,18 +622,24 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             rh[i] = __builtin_amdgcn_raw_buffer_load_b128(hr, ha, state_at(2 * (i % 2), 0, i / 2) * 2, 0);
         }
         const size_t sp0 = (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
-        const auto lr = rsrc(a.lc + sp0, live ? FQ * 4 : 0), dr = rsrc(a.dtv + sp0, live ? FQ * 4 : 0);
-        const uint32_t tt = tid % FQ;
+        const uint32_t some = live ? FQ * 4 : 0, tt = tid % FQ;
+        const auto lr = rsrc(a.lc + sp0, some), dr = rsrc(a.dtv + sp0, some), sr = rsrc(a.slope + sp0, some);
         auto one = [](auto r, uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * at, 0, 0)); };
         rl = one(lr, tt);
         rt = one(lr, FQ - 1);
         rr = one(lr, tt >= 16 ? tt / 16 * 16 - 1 : 0);      // (token blocks past the first)
         rd = one(dr, tt);
+        rs = one(sr, tt);
+        ra = __builtin_amdgcn_raw_buffer_load_b16(rsrc((const bf16*)a.A_log + h, 2), 0, 0, 0);
+        rD = __builtin_amdgcn_raw_buffer_load_b16(rsrc((const bf16*)a.D + h, a.D ? 2 : 0), 0, 0, 0);
     };
 
     // C B^T, lower tiles
     auto row8 = [&](const bf16* p, uint32_t t, int at) {
         return t < tl ? *reinterpret_cast<const s8v*>(p + t * gn + at) : s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    };
+    auto row4 = [&](const bf16* p, uint32_t t, int at) {
+        return t < tl ? *reinterpret_cast<const s4v*>(p + t * gn + at) : s4v{0, 0, 0, 0};
     };
     for (int i = w; i < F_TILES; i += 8) {
         int T = 0;
@@ -632,28 +653,68 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         SS[i * WAVE + lane] = floatx4{0, 0, 0, 0};
     }
     RS[w][lane] = RS[w][lane + 64] = 0.0f;      // sinks before the wave's sources stay 0
+    // B of the wave's sources; k = n in the order 4 q .. + 3, 16 + 4 q .. + 3 of
+    // each 32, in which the transposing loads of the other operand meet no
+    // bank twice
     s8v bf[4];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) bf[ks] = row8(Bg, 16 * J + li, 32 * ks + 8 * lq);
-    u32x2 cp[8];                                 // C[t = 16 T + 4 lq + r][n = 16 w + li]
+    for (int ks = 0; ks < 4; ++ks) bf[ks] = cat8(row4(Bg, 16 * J + li, 32 * ks + 4 * lq), row4(Bg, 16 * J + li, 32 * ks + 16 + 4 * lq));
+    s4v cp[8];                                   // C[t = 16 T + li][n = 16 w + 4 lq + r]
 #pragma unroll
-    for (int T = 0; T < 8; ++T)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint32_t x = 0;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint32_t t = 16 * T + 4 * lq + 2 * k + r;
-                if (t < tl) x |= (uint32_t)*reinterpret_cast<const uint16_t*>(Cg + t * gn + 16 * w + li) << (16 * r);
-            }
-            cp[T][k] = x;
-            __builtin_amdgcn_sched_barrier(0);
-        }
+    for (int T = 0; T < 8; ++T) cp[T] = row4(Cg, 16 * T + li, 16 * w + 4 * lq);
 
-    floatx4 dc[8], db[8];
+    floatx4 dc[8], db[8];                        // [n = 16 w + 4 lq + r][t = 16 T + li]
 #pragma unroll
     for (int T = 0; T < 8; ++T) dc[T] = db[T] = floatx4{0, 0, 0, 0};
     if (v_first < v_end) fetch(v_first, true);
+
+    // a_t: pairs of a source before t and a sink from t on; lane l has tokens
+    // 2 l and 2 l + 1.  The wave with the fewest tiles gathers a pair's sums and
+    // finishes them while the others work on the next.
+    constexpr int TAIL = 4;
+    float pre[2], suf[2], dir[2], tdt[2], tsl[2], tedge = 0.0f, tdd = 0.0f, tA = 0.0f;
+    auto gather = [&]() {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int t = 2 * lane + k;
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += VO[i][t];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += RS[i][t];
+            const float dt = DT[t], u = UO[t], cs = CS[t];
+            tsl[k] = SL[t];
+            tdt[k] = dt;
+            dir[k] = u + cs;
+            pre[k] = dt * u;
+            suf[k] = s - dt * cs;
+        }
+        tedge = tdd = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            tedge += red[i][0];
+            tdd += red[i][1];
+        }
+        tedge *= EL[FQ - 1];
+    };
+    auto finish = [&](uint32_t v) {
+        const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
+        const float both = pre[0] + pre[1], own = suf[0] + suf[1];
+        const float p_in = tedge + (wave_prefix_sum(both) - both);
+        const float s_from = wave_sum(own) - wave_prefix_sum(own);      // behind this lane's
+        const float da0 = p_in + (s_from + own), da1 = (p_in + pre[0]) + (s_from + suf[1]);
+        const float q0 = fmaf(tA, da0, dir[0]) * tsl[0], q1 = fmaf(tA, da1, dir[1]) * tsl[1];
+        float* q = a.q + (((size_t)sl * a.batch + b) * a.H + h) * L + t0;
+        if (2 * lane < (int)tl) q[2 * lane] = q0;
+        if (2 * lane + 1 < (int)tl) q[2 * lane + 1] = q1;
+        const float dA = wave_sum(tdt[0] * da0 + tdt[1] * da1), dq = wave_sum(q0 + q1);
+        if (lane == 0) {
+            float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 3;
+            o[0] = dq;
+            o[1] = tA * dA;
+            o[2] = tdd;
+        }
+    };
 
     for (uint32_t v = v_first; v < v_end; ++v) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
@@ -675,6 +736,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             const uint32_t j = tid + i * F_NT, pc = j / 32 % 2, nt = j / 64 % (FN / 16), pt = j / 64 / (FN / 16);
             *reinterpret_cast<u32x4*>((pc ? Gl : Gh) + (16 * nt + j % 32 / 2) * FXP + 16 * pt + 8 * (j % 2)) = rg[i];
         }
+        const float D = val((short)rD), A_h = -__expf(val((short)ra));
         if (tid < FQ) {
             const float er = __expf(rt - rl);
             LC[tid] = rl;
@@ -683,37 +745,42 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             ER[tid] = er;
             WB[tid] = rd * er;
             AF[tid] = __expf(rl - rr);
+            SL[tid] = rs;
         }
         lds_barrier();
+        if (w == TAIL && v > v_first) finish(v - 1);
+        tA = A_h;
 
-        // dB: x and G1 (k = row)
+        // dB^T [n][source]: G1 and x (k = row); <G1, h0> as a trace
         s8v gf[4], hf[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             gf[i] = *reinterpret_cast<const s8v*>((i / 2 ? Gl : Gh) + (16 * w + li) * FXP + 32 * (i % 2) + 8 * lq);
             hf[i] = __builtin_bit_cast(s8v, rh[i]);
         }
-        float gh = 0.0f;
+        floatx4 tr{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                gh = fmaf(val(gf[i][e]) + val(gf[i + 2][e]), val(hf[i][e]) + val(hf[i + 2][e]), gh);
-        gh = wave_sum(gh);
+        for (int ks = 0; ks < 2; ++ks) {
+            tr = mma(gf[ks], hf[ks], tr);
+            tr = mma(gf[ks], hf[ks + 2], tr);
+            tr = mma(gf[ks + 2], hf[ks], tr);
+        }
 #pragma unroll
         for (int T = 0; T < 8; ++T) {
             const bf16* xp = Xs + (16 * T + li) * FXP + 8 * lq;
             const s8v x0 = *reinterpret_cast<const s8v*>(xp), x1 = *reinterpret_cast<const s8v*>(xp + 32);
             floatx4 y{0, 0, 0, 0};
-            y = mma(x0, gf[0], y);
-            y = mma(x1, gf[1], y);
-            y = mma(x0, gf[2], y);
-            y = mma(x1, gf[3], y);
-            const floatx4 wb = *reinterpret_cast<const floatx4*>(WB + 16 * T + 4 * lq);
+            y = mma(gf[0], x0, y);
+            y = mma(gf[1], x1, y);
+            y = mma(gf[2], x0, y);
+            y = mma(gf[3], x1, y);
+            const float wb = WB[16 * T + li];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) db[T][r] = fmaf(wb[r], y[r], db[T][r]);
-            if (T % 2) __builtin_amdgcn_sched_barrier(0);
+            for (int r = 0; r < 4; ++r) db[T][r] = fmaf(wb, y[r], db[T][r]);
         }
+        float gh = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) gh += 4 * lq + r == li ? tr[r] : 0.0f;
 
         // dx'^T [row][source] from G1 and B (k = n)
         const int j = 16 * J + li;
@@ -724,10 +791,9 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                const int at = (32 * ks + 8 * lq + tk) * FXP + 16 * p + 4 * tc;
-                dx[p] = mma(cat8(ld_tr(Gh + at), ld_tr(Gh + at + 4 * FXP)), bf[ks], dx[p]);
-                dx[p] = mma(cat8(ld_tr(Gl + at), ld_tr(Gl + at + 4 * FXP)), bf[ks], dx[p]);
-                if (p % 2) __builtin_amdgcn_sched_barrier(0);
+                const int at = (32 * ks + 4 * lq + tk) * FXP + 16 * p + 4 * tc;
+                dx[p] = mma(cat8(ld_tr(Gh + at), ld_tr(Gh + at + 16 * FXP)), bf[ks], dx[p]);
+                dx[p] = mma(cat8(ld_tr(Gl + at), ld_tr(Gl + at + 16 * FXP)), bf[ks], dx[p]);
             }
         const float erj = ER[j], dtj = DT[j], lcj = LC[j];
         float uo = 0.0f;
@@ -742,7 +808,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         }
         uo = swap_add32(swap_add16(uo));
 
-        // sinks T: dC of all sources before the chunk; S and M of column J
+        // sinks T: dC^T [n][sink] of all sources before the chunk; S and M of column J
         const s8v xj0 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 8 * lq);
         const s8v xj1 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 32 + 8 * lq);
         float col = 0.0f, diag = 0.0f;
@@ -755,19 +821,19 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 const bf16* yp = Ys + (16 * T + li) * FXP + 8 * lq;
                 const s8v y0 = *reinterpret_cast<const s8v*>(yp), y1 = *reinterpret_cast<const s8v*>(yp + 32);
                 floatx4 x{0, 0, 0, 0};
-                x = mma(y0, hf[0], x);
-                x = mma(y1, hf[1], x);
-                x = mma(y0, hf[2], x);
-                x = mma(y1, hf[3], x);
-                const floatx4 el = *reinterpret_cast<const floatx4*>(EL + 16 * T + 4 * lq);
-                floatx4 vo;
+                x = mma(hf[0], y0, x);
+                x = mma(hf[1], y1, x);
+                x = mma(hf[2], y0, x);
+                x = mma(hf[3], y1, x);
+                const float el = EL[16 * T + li];
+                float vo = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float d = el[r] * x[r];
-                    dc[T][r] += d;
-                    vo[r] = group_sum<16>(d * __uint_as_float(r & 1 ? cp[T][r / 2] & 0xffff0000u : cp[T][r / 2] << 16));
+                    dc[T][r] = fmaf(el, x[r], dc[T][r]);
+                    vo = fmaf(x[r], val(cp[T][r]), vo);
                 }
-                if (li == 0) *reinterpret_cast<floatx4*>(&VO[w][16 * T + 4 * lq]) = vo;
+                vo = el * swap_add32(swap_add16(vo));
+                if (lq == 0) VO[w][16 * T + li] = vo;
                 mh[k] = ml[k] = s4v{0, 0, 0, 0};
                 if (T >= J) {
                     floatx4 sd{0, 0, 0, 0};
@@ -790,14 +856,15 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                     floatx4 ss = SS[id * WAVE + lane], m, row;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
+                        const float se = sd[r] * e[r], sdt = se * dtj;
                         m[r] = cb[r] * e[r];
-                        ss[r] = fmaf(sd[r] * e[r], dtj, ss[r]);
-                        const float kk = sd[r] * m[r];
-                        col += kk;
-                        row[r] = group_sum<16>(kk * dtj);
+                        ss[r] += sdt;
+                        col = fmaf(se, cb[r], col);
+                        row[r] = sdt * cb[r];
                     }
                     SS[id * WAVE + lane] = ss;
-                    if (li == 0) *reinterpret_cast<floatx4*>(&RS[w][16 * T + 4 * lq]) = row;
+                    const float rsum = row_sums4(row);
+                    if (li < 4) RS[w][16 * T + 4 * lq + li] = rsum;
                     mh[k] = take4(m);
                     ml[k] = take4(m);
                 }
@@ -818,12 +885,12 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             UO[j] = uo;
             CS[j] = col;
         }
+        gh = wave_sum(gh);
         diag = wave_sum(diag);
         if (lane == 0) {
             red[w][0] = gh;
             red[w][1] = diag;
         }
-        const float D = a.D ? to_f(((const bf16*)a.D)[h]) : 0.0f;
         bf16* out0 = (bf16*)a.dX + ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
         const uint32_t out = j * (uint32_t)hp + 4 * lq;
 #pragma unroll
@@ -838,51 +905,9 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         // nothing that was issued later
         fetch(min(v + 1, v_end - 1), v + 1 < v_end);
         lds_barrier();
-        // a_t: pairs of a source before t and a sink from t on; lane l has
-        // tokens 2 l and 2 l + 1
-        if (w == 7) {
-            float pre[2], suf[2], dir[2], dt[2], slope[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int t = 2 * lane + k;
-                float s = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += VO[i][t];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += RS[i][t];
-                slope[k] = a.slope[(((size_t)b * a.H + h) * a.nchunk + c) * FQ + t];
-                dt[k] = DT[t];
-                dir[k] = UO[t] + CS[t];
-                pre[k] = dt[k] * UO[t];
-                suf[k] = s - dt[k] * CS[t];
-            }
-            const float both = pre[0] + pre[1], own = suf[0] + suf[1];
-            const float p_in = wave_prefix_sum(both) - both;
-            const float s_all = wave_sum(own), s_from = s_all - wave_prefix_sum(own);   // behind this lane's
-            float e0 = 0.0f, dd = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e0 += red[i][0];
-                dd += red[i][1];
-            }
-            const float edge = __expf(LC[FQ - 1]) * e0, A = -expf(to_f(((const bf16*)a.A_log)[h]));
-            float da[2], q[2];
-            da[0] = edge + p_in + (s_from + own);
-            da[1] = edge + (p_in + pre[0]) + (s_from + suf[1]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                q[k] = (dir[k] + A * da[k]) * slope[k];
-                if (2 * lane + k < (int)tl) a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + 2 * lane + k] = q[k];
-            }
-            const float dA = wave_sum(dt[0] * da[0] + dt[1] * da[1]), dq = wave_sum(q[0] + q[1]);
-            if (lane == 0) {
-                float* o = a.part + ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * 3;
-                o[0] = dq;
-                o[1] = A * dA;
-                o[2] = dd;
-            }
-        }
+        if (w == TAIL) gather();
     }
+    if (w == TAIL && v_first < v_end) finish(v_end - 1);
 
     // within the chunk: sum of S over the share's heads with B and C
     lds_barrier();
@@ -910,8 +935,8 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                     lo[e] = take4(x);
                 }
                 const s8v ct = cat8(ld_tr(tp), ld_tr(tp + 16 * FBP));
-                db[T] = mma(cat8(hi[0], hi[1]), ct, db[T]);
-                db[T] = mma(cat8(lo[0], lo[1]), ct, db[T]);
+                db[T] = mma(ct, cat8(hi[0], hi[1]), db[T]);
+                db[T] = mma(ct, cat8(lo[0], lo[1]), db[T]);
             }
             if (k <= T) {
                 const bf16* bp = (Bs + (16 * k + 4 * lq + tk) * FBP + 16 * w + 4 * tc);
@@ -927,19 +952,16 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                     lo[e] = take4(x);
                 }
                 const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 16 * FBP));
-                dc[T] = mma(cat8(hi[0], hi[1]), bt, dc[T]);
-                dc[T] = mma(cat8(lo[0], lo[1]), bt, dc[T]);
+                dc[T] = mma(bt, cat8(hi[0], hi[1]), dc[T]);
+                dc[T] = mma(bt, cat8(lo[0], lo[1]), dc[T]);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t t = 16 * T + 4 * lq + r;
-            if (t < tl) {
-                const size_t at = (size_t)sp * a.share + (((size_t)b * L + t0 + t) * a.G + g) * FN + 16 * w + li;
-                a.cpart[at] = dc[T][r];
-                a.bpart[at] = db[T][r];
-            }
+        const uint32_t t = 16 * T + li;
+        if (t < tl) {
+            const size_t at = (size_t)sp * a.share + (((size_t)b * L + t0 + t) * a.G + g) * FN + 16 * w + 4 * lq;
+            *reinterpret_cast<floatx4*>(a.cpart + at) = dc[T];
+            *reinterpret_cast<floatx4*>(a.bpart + at) = db[T];
         }
     }
 }
