@@ -420,13 +420,6 @@ __global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
     a.slope[at] = c * FQ + t < a.L ? dt_slope<bf16>(a, b, c * FQ + t, h) : 0.0f;
 }
 
-// 16-byte piece i of a tile of FQ rows, `per` pieces a row: zeros behind the
-// rows there are
-__device__ __forceinline__ u32x4 piece(const bf16* src, size_t stride, uint32_t rows, uint32_t per, uint32_t i) {
-    const uint32_t r = i / per, c = i % per;
-    return r < rows ? *reinterpret_cast<const u32x4*>(src + r * stride + 8 * c) : u32x4{0, 0, 0, 0};
-}
-
 // where tile (row tile, column tile) of a kept state's piece starts
 __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt, uint32_t piece) {
     return ((pt * (FN / 16) + nt) * 2 + piece) * 256;
@@ -634,39 +627,65 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         rD = __builtin_amdgcn_raw_buffer_load_b16(rsrc((const bf16*)a.D + h, a.D ? 2 : 0), 0, 0, 0);
     };
 
-    // C B^T, lower tiles
-    auto row8 = [&](const bf16* p, uint32_t t, int at) {
-        return t < tl ? *reinterpret_cast<const s8v*>(p + t * gn + at) : s8v{0, 0, 0, 0, 0, 0, 0, 0};
+    auto touch = [&](uint32_t v, uint32_t (&out)[2]) {
+        const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice, r = min(tid % FQ, tl - 1);
+        const size_t row = ((size_t)b * L + t0 + r) * hp + (size_t)h * P + sl * FP;
+        const size_t slot = ((((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk + c) * (2 * FN * FP);
+        const bf16* first = tid < 2 * FQ ? (const bf16*)(tid < FQ ? a.X : a.dY) + row : (const bf16*)a.gst + slot + 64 * (tid - 2 * FQ);
+        out[0] = *reinterpret_cast<const uint32_t*>(first);
+        out[1] = *reinterpret_cast<const uint32_t*>((const bf16*)a.hst + slot + 64 * (tid % 256));
     };
-    auto row4 = [&](const bf16* p, uint32_t t, int at) {
-        return t < tl ? *reinterpret_cast<const s4v*>(p + t * gn + at) : s4v{0, 0, 0, 0};
+    if (v_first < v_end) fetch(v_first, true);
+
+    // B and C once through LDS: C B^T (lower tiles), B of the wave's sources, C
+    // of its columns
+    bf16 *Bs = stage, *Cs = stage + FQ * FBP;
+    static_assert(2 * FBP <= 4 * FXP, "B and C fit where the pairs' tiles are");
+    auto stage_bc = [&]() {
+        const auto br = rsrc(Bg, ((tl - 1) * a.G * FN + FN) * 2), cr = rsrc(Cg, ((tl - 1) * a.G * FN + FN) * 2);
+        u32x4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t j = tid + i * F_NT, at = j / (FN / 8) * (a.G * FN * 2) + j % (FN / 8) * 16;
+            x[i] = __builtin_amdgcn_raw_buffer_load_b128(br, at, 0, 0);
+            y[i] = __builtin_amdgcn_raw_buffer_load_b128(cr, at, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t j = tid + i * F_NT, at = j / (FN / 8) * FBP + j % (FN / 8) * 8;
+            *reinterpret_cast<u32x4*>(Bs + at) = x[i];
+            *reinterpret_cast<u32x4*>(Cs + at) = y[i];
+        }
     };
+    stage_bc();
+    lds_barrier();
     for (int i = w; i < F_TILES; i += 8) {
         int T = 0;
         while (tile_of(T + 1, 0) <= i) ++T;
-        const int Jc = i - tile_of(T, 0);
+        const bf16 *cr = Cs + (16 * T + li) * FBP + 8 * lq, *br = Bs + (16 * (i - tile_of(T, 0)) + li) * FBP + 8 * lq;
         floatx4 acc{0, 0, 0, 0};
 #pragma unroll
         for (int ks = 0; ks < FN / 32; ++ks)
-            acc = mma(row8(Cg, 16 * T + li, 32 * ks + 8 * lq), row8(Bg, 16 * Jc + li, 32 * ks + 8 * lq), acc);
+            acc = mma(*reinterpret_cast<const s8v*>(cr + 32 * ks), *reinterpret_cast<const s8v*>(br + 32 * ks), acc);
         CB[i * WAVE + lane] = acc;
         SS[i * WAVE + lane] = floatx4{0, 0, 0, 0};
     }
     RS[w][lane] = RS[w][lane + 64] = 0.0f;      // sinks before the wave's sources stay 0
-    // B of the wave's sources; k = n in the order 4 q .. + 3, 16 + 4 q .. + 3 of
-    // each 32, in which the transposing loads of the other operand meet no
-    // bank twice
+    // k = n in the order 4 q .. + 3, 16 + 4 q .. + 3 of each 32, in which the
+    // transposing loads of the other operand meet no bank twice
     s8v bf[4];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) bf[ks] = cat8(row4(Bg, 16 * J + li, 32 * ks + 4 * lq), row4(Bg, 16 * J + li, 32 * ks + 16 + 4 * lq));
+    for (int ks = 0; ks < 4; ++ks) {
+        const bf16* br = Bs + (16 * J + li) * FBP + 32 * ks + 4 * lq;
+        bf[ks] = cat8(*reinterpret_cast<const s4v*>(br), *reinterpret_cast<const s4v*>(br + 16));
+    }
     s4v cp[8];                                   // C[t = 16 T + li][n = 16 w + 4 lq + r]
 #pragma unroll
-    for (int T = 0; T < 8; ++T) cp[T] = row4(Cg, 16 * T + li, 16 * w + 4 * lq);
+    for (int T = 0; T < 8; ++T) cp[T] = *reinterpret_cast<const s4v*>(Cs + (16 * T + li) * FBP + 16 * w + 4 * lq);
 
     floatx4 dc[8], db[8];                        // [n = 16 w + 4 lq + r][t = 16 T + li]
 #pragma unroll
     for (int T = 0; T < 8; ++T) dc[T] = db[T] = floatx4{0, 0, 0, 0};
-    if (v_first < v_end) fetch(v_first, true);
 
     // a_t: pairs of a source before t and a sink from t on; lane l has tokens
     // 2 l and 2 l + 1.  The wave with the fewest tiles gathers a pair's sums and
@@ -748,6 +767,10 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
             SL[tid] = rs;
         }
         lds_barrier();
+        // one word of each line of the next pair's rows and states, long before
+        // the registers that take them are free: they come from the L2 then
+        uint32_t touched[2] = {0, 0};
+        if (v + 1 < v_end) touch(v + 1, touched);
         if (w == TAIL && v > v_first) finish(v - 1);
         tA = A_h;
 
@@ -903,6 +926,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         }
         // behind the stores: waiting for the next pair at the top waits for
         // nothing that was issued later
+        asm volatile("" ::"v"(touched[0]), "v"(touched[1]));
         fetch(min(v + 1, v_end - 1), v + 1 < v_end);
         lds_barrier();
         if (w == TAIL) gather();
@@ -911,12 +935,7 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
 
     // within the chunk: sum of S over the share's heads with B and C
     lds_barrier();
-    bf16 *Bs = stage, *Cs = stage + FQ * FBP;
-    static_assert(2 * FBP <= 4 * FXP, "B and C fit where the pairs' tiles were");
-    for (uint32_t i = tid; i < FQ * FN / 8; i += F_NT) {
-        *reinterpret_cast<u32x4*>(Bs + i / (FN / 8) * FBP + i % (FN / 8) * 8) = piece(Bg, gn, tl, FN / 8, i);
-        *reinterpret_cast<u32x4*>(Cs + i / (FN / 8) * FBP + i % (FN / 8) * 8) = piece(Cg, gn, tl, FN / 8, i);
-    }
+    stage_bc();
     lds_barrier();
     const float* Sf = reinterpret_cast<const float*>(SS);
 #pragma unroll
@@ -1089,7 +1108,7 @@ Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
 }
 // (a chunk's rows within 32-bit byte offsets)
 bool fast_dims(const lssm_ssd_dims& d, int act) {
-    return act == LSSM_BF16 && d.N == FN && d.P % FP == 0 && (uint64_t)d.H * d.P * FQ * 2 < (1u << 31);
+    return act == LSSM_BF16 && d.N == FN && d.P % FP == 0 && (uint64_t)d.H * std::max(d.P, d.N) * FQ * 2 < (1u << 31);
 }
 
 template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArgs& a) {
