@@ -24,12 +24,11 @@
 //   K[s, j] = (dy_s.x_j)(C_s.B_j) E dt_j
 // which adds terms of one chunk only: no sum over the whole sequence cancels.
 //
-// Three steps: a walk over the chunks keeps the states h0 (forwards) and G1
-// (backwards) of every chunk; the chunks' gradients, in parallel; sums over
-// heads, slices and chunks.  Every order of summation is fixed.
+// Three steps: the states h0 (forwards) and G1 (backwards) of every chunk are
+// kept; the chunks' gradients, in parallel; sums over heads, slices and chunks.
+// Every order of summation is fixed.
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 #include <type_traits>
 
 #include "common.hpp"
@@ -46,6 +45,7 @@ __device__ __forceinline__ floatx4 mma4(float a, float b, floatx4 c) {
 // ---------------------------------------------------------------------------
 // Any type, head size and state size (N <= 256), fp32 products
 // (v_mfma_f32_16x16x4_f32): chunks of 32 tokens, slices of 32 state rows.
+// Every chunk's own state in parallel, then the scan over the chunks, in place.
 // The sums of A dt are held in 64 bits: differences of sums that grow along a
 // chunk are what every decay is the exponential of.
 // ---------------------------------------------------------------------------
@@ -54,8 +54,7 @@ constexpr int GP = 32;      // state rows a slice
 constexpr int GXP = 36;     // LDS pitch of a [token][row] tile (= 4 modulo 64 banks x 9)
 constexpr int G_NT = 256;
 
-// gradient of raw + bias from that of dt: the softplus' slope, 0 where the
-// clamp holds
+// slope of dt in raw + bias: the softplus', 0 where the clamp holds
 template <typename T> __device__ __forceinline__ float dt_slope(const SsdBwdArgs& a, uint32_t b, uint32_t t, uint32_t h) {
     const float v = to_f(((const T*)a.dt)[((size_t)b * a.L + t) * a.H + h]) + to_f(((const T*)a.dt_bias)[h]);
     const float sp = v > 20.0f ? v : log1pf(expf(v));
@@ -69,96 +68,128 @@ struct Steps { double lc, tot; float dt; };
 template <typename T> __device__ __forceinline__ Steps chunk_steps(const SsdBwdArgs& a, uint32_t b, uint32_t h, uint32_t t0,
                                                                    uint32_t tl) {
     const uint32_t t = threadIdx.x % WAVE;
-    const double A = -exp((double)to_f(((const T*)a.A_log)[h]));
-    double dt = 0.0;
+    const float A = -expf(to_f(((const T*)a.A_log)[h]));
+    float dt = 0.0f;
     if (t < tl) {
-        const double v = (double)to_f(((const T*)a.dt)[((size_t)b * a.L + t0 + t) * a.H + h]) +
-                         (double)to_f(((const T*)a.dt_bias)[h]);
-        dt = v > 40.0 ? v : log1p(exp(v));
-        dt = fmin(fmax(dt, (double)a.dt_min), (double)a.dt_max);
+        const float v = to_f(((const T*)a.dt)[((size_t)b * a.L + t0 + t) * a.H + h]) + to_f(((const T*)a.dt_bias)[h]);
+        dt = v > 20.0f ? v : log1pf(expf(v));
+        dt = fminf(fmaxf(dt, a.dt_min), a.dt_max);
     }
-    double s = A * dt;
+    double s = (double)A * (double)dt;
 #pragma unroll
     for (int d = 1; d < GQ; d <<= 1) {
         const double o = __shfl_up(s, d);
         if ((int)t >= d) s += o;
     }
-    return {s, __shfl(s, GQ - 1), (float)dt};
+    return {s, __shfl(s, GQ - 1), dt};
 }
 
-// rows t0 .. t0 + tl of a [rows][stride] array, columns c0 .. c0 + n, into
-// LDS [GQ][pitch], zeros behind the ends (W columns in all)
+// rows 0 .. rows - 1 of a [rows][stride] array, n columns, into LDS
+// [GQ][pitch] (pitch a multiple of four), zeros behind the ends (W columns in
+// all); 16 bytes at a time where the rows are whole and aligned
 template <typename T, int W> __device__ __forceinline__ void load_tile(float* dst, int pitch, const T* src, size_t stride,
                                                                        uint32_t rows, uint32_t n) {
+    constexpr int E = 16 / sizeof(T);
+    if (n == W && (((uintptr_t)src | (stride * sizeof(T))) & 15) == 0) {
+        typedef T TE __attribute__((ext_vector_type(E)));
+#pragma unroll
+        for (uint32_t k = 0; k < (GQ * W / E + G_NT - 1) / G_NT; ++k) {
+            const uint32_t i = threadIdx.x + k * G_NT, r = i / (W / E), c = i % (W / E) * E;
+            if (GQ * W / E % G_NT && i >= GQ * W / E) break;
+            TE v = TE(0);
+            if (r < rows) v = *reinterpret_cast<const TE*>(src + r * stride + c);
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+                *reinterpret_cast<floatx4*>(dst + r * pitch + c + e) = floatx4{to_f(v[e]), to_f(v[e + 1]), to_f(v[e + 2]), to_f(v[e + 3])};
+        }
+        return;
+    }
     for (uint32_t i = threadIdx.x; i < GQ * W; i += G_NT) {
         const uint32_t r = i / W, c = i % W;
         dst[r * pitch + c] = (r < rows && c < n) ? to_f(src[r * stride + c]) : 0.0f;
     }
 }
 
-// The walk: block (head, slice), sequence, direction.  Direction 0 keeps h0 of
-// every chunk, 1 its G1; both add to the state weighted outer products of the
-// chunk's rows (x with B, dy with C).
-template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_walk_kernel(SsdBwdArgs a) {
+// What a chunk alone adds to the state behind it (direction 0: weighted outer
+// products of x with B) or to the gradient in front of it (1: of dy with C):
+// block (head, slice and direction; chunk; sequence).
+template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_own_kernel(SsdBwdArgs a) {
     constexpr int NP = NT + 4, TN = NT / 64;
-    __shared__ float Rs[GQ * GXP], Cs[GQ * NP], W[GQ], Dq;
-    const uint32_t h = blockIdx.x / a.nslice, p0 = blockIdx.x % a.nslice * GP, b = blockIdx.y;
-    const bool back = blockIdx.z != 0;
-    const uint32_t P = a.P, N = a.N, L = a.L, pn = min((uint32_t)GP, P - p0);
+    __shared__ __attribute__((aligned(16))) float Rs[GQ * GXP], Cs[GQ * NP], W[GQ];
+    const uint32_t c = blockIdx.y, h = blockIdx.x / 2 / a.nslice, sl = blockIdx.x / 2 % a.nslice, p0 = sl * GP;
+    const uint32_t b = blockIdx.z;
+    const bool back = blockIdx.x % 2 != 0;
+    const uint32_t P = a.P, N = a.N, L = a.L, pn = min((uint32_t)GP, P - p0), t0 = c * GQ, tl = min((uint32_t)GQ, L - t0);
     const uint32_t g = h / (a.H / a.G);
     const int tid = threadIdx.x, lane = tid % WAVE, li = lane % 16, lq = lane / 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const float* init = back ? a.d_state : a.state;
-    float* slots = (back ? a.gst : a.hst) + ((size_t)b * a.H + h) * a.nchunk * P * N;
-    floatx4 s[2][TN];
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t p = 16 * pt + 4 * lq + r, n = 16 * (w + 4 * i) + li;
-                    s[pt][i][r] = (p < pn && n < N) ? f(s[pt][i][r], (size_t)(p0 + p) * N + n) : 0.0f;
-                }
-    };
-    each([&](float, size_t at) { return init ? init[((size_t)b * a.H + h) * P * N + at] : 0.0f; });
-    for (uint32_t k = 0; k < a.nchunk; ++k) {
-        const uint32_t c = back ? a.nchunk - 1 - k : k, t0 = c * GQ, tl = min((uint32_t)GQ, L - t0);
-        each([&](float v, size_t at) { return slots[(size_t)c * P * N + at] = v; });
-        __syncthreads();
-        load_tile<T, GP>(Rs, GXP, (const T*)(back ? a.dY : a.X) + ((size_t)b * L + t0) * a.H * P + (size_t)h * P + p0,
-                         (size_t)a.H * P, tl, pn);
-        load_tile<T, NT>(Cs, NP, (const T*)(back ? a.C : a.B) + ((size_t)b * L + t0) * a.G * N + (size_t)g * N,
-                         (size_t)a.G * N, tl, N);
-        if (w == 0) {
-            const Steps st = chunk_steps<T>(a, b, h, t0, tl);
-            if (lane < GQ) W[lane] = back ? (float)exp(st.lc) : st.dt * (float)exp(st.tot - st.lc);
-            if (lane == 0) Dq = (float)exp(st.tot);
-        }
-        __syncthreads();
-        const float dq = Dq;
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-            for (int i = 0; i < TN; ++i) {
-                s[pt][i] *= dq;
-#pragma unroll
-                for (int kk = 0; kk < GQ / 4; ++kk) {
-                    const int t = 4 * kk + lq;
-                    s[pt][i] = mma4(Rs[t * GXP + 16 * pt + li] * W[t], Cs[t * NP + 16 * (w + 4 * i) + li], s[pt][i]);
-                }
-            }
+    load_tile<T, GP>(Rs, GXP, (const T*)(back ? a.dY : a.X) + ((size_t)b * L + t0) * a.H * P + (size_t)h * P + p0,
+                     (size_t)a.H * P, tl, pn);
+    load_tile<T, NT>(Cs, NP, (const T*)(back ? a.C : a.B) + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl,
+                     N);
+    if (w == 0) {
+        const Steps st = chunk_steps<T>(a, b, h, t0, tl);
+        if (lane < GQ) W[lane] = back ? expf((float)st.lc) : st.dt * expf((float)(st.tot - st.lc));
+        if (lane == 0 && !back && sl == 0) a.lc[((size_t)b * a.H + h) * a.nchunk + c] = expf((float)st.tot);
     }
-    if (back && a.d_state0) each([&](float v, size_t at) { return a.d_state0[((size_t)b * a.H + h) * P * N + at] = v; });
+    __syncthreads();
+    float* own = (back ? a.gst : a.hst) + (((size_t)b * a.H + h) * a.nchunk + c) * P * N;
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const uint32_t n = 16 * (w + 4 * i) + li;
+            floatx4 s{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < GQ / 4; ++k) {
+                const int t = 4 * k + lq;
+                s = mma4(Rs[t * GXP + 16 * pt + li] * W[t], Cs[t * NP + n], s);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t p = 16 * pt + 4 * lq + r;
+                if (p < pn && n < N) own[(size_t)(p0 + p) * N + n] = s[r];
+            }
+        }
+}
+
+// The scan: an element of a head's state a thread.  Slot c holds what chunk c
+// adds and gets the state that enters it (direction 0), or the gradient of the
+// one that leaves it (1).  Slots are read SC ahead.
+constexpr int SC = 8;
+__global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
+    const uint32_t PN = a.P * a.N, i = blockIdx.x / 2 * G_NT + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const bool back = blockIdx.x % 2 != 0;
+    if (i >= PN) return;
+    const size_t bh = (size_t)b * a.H + h;
+    float* slots = (back ? a.gst : a.hst) + bh * a.nchunk * PN + i;
+    const float* decay = a.lc + bh * a.nchunk;
+    const float* init = back ? a.d_state : a.state;
+    float s = init ? init[bh * PN + i] : 0.0f;
+    for (uint32_t k0 = 0; k0 < a.nchunk; k0 += SC) {
+        float own[SC], d[SC];
+#pragma unroll
+        for (int k = 0; k < SC; ++k) {
+            const uint32_t q = min(k0 + k, a.nchunk - 1), c = back ? a.nchunk - 1 - q : q;
+            own[k] = slots[(size_t)c * PN];
+            d[k] = decay[c];
+        }
+#pragma unroll
+        for (int k = 0; k < SC; ++k) {
+            if (k0 + k >= a.nchunk) break;
+            slots[(size_t)(back ? a.nchunk - 1 - (k0 + k) : k0 + k) * PN] = s;
+            s = fmaf(d[k], s, own[k]);
+        }
+    }
+    if (back && a.d_state0) a.d_state0[bh * PN + i] = s;
 }
 
 // The chunks' gradients: block = chunk, sequence, group, share of the group's
 // (head, slice) pairs.  dB and dC of the share stay in registers.
 template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
     constexpr int NP = NT + 4, TN = NT / 64;
-    __shared__ float Bs[GQ * NP], Cs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
-    __shared__ float Xs[GQ * GXP], Ys[GQ * GXP], Ms[GQ * GXP];
+    __shared__ __attribute__((aligned(16))) float Bs[GQ * NP], Cs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
+    __shared__ __attribute__((aligned(16))) float Xs[GQ * GXP], Ys[GQ * GXP], Ms[GQ * GXP];
     __shared__ double Lc[GQ];
     __shared__ float DT[GQ], EL[GQ], ER[GQ], RS[2][GQ], CS[2][GQ], VO[4][GQ], UO[2][GQ], red[4][2];
     const uint32_t P = a.P, N = a.N, L = a.L, hpg = a.H / a.G;
@@ -199,8 +230,8 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
             if (lane < GQ) {
                 Lc[lane] = st.lc;
                 DT[lane] = st.dt;
-                EL[lane] = (float)exp(st.lc);
-                ER[lane] = (float)exp(st.tot - st.lc);
+                EL[lane] = expf((float)st.lc);
+                ER[lane] = expf((float)(st.tot - st.lc));
             }
         }
         __syncthreads();
@@ -295,7 +326,7 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
                 if (lane >= d) pre += x;
                 if (lane + d < GQ) suf += y;
             }
-            const float edge = (float)exp(tot) * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
+            const float edge = expf((float)tot) * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
             const float da = edge + (pre - own) + suf;
             const float A = -expf(to_f(((const T*)a.A_log)[h]));
             float q = 0.0f;
@@ -431,8 +462,8 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // 16 columns ([row tile][column tile][piece][n][row]): what a wave stores at
 // once is contiguous (32 bytes of each of four waves to a line stored at 3.0
 // TB/s), and a lane of the chunks' kernel finds its operand in 16 bytes.
-constexpr int W_NT = 256;
-template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
+constexpr int W_NT = 256, NC = 64;
+__global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
     constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 16;
     constexpr int XV = FQ * FP / 8 / W_NT, BV = FQ * NC / 8 / W_NT;     // 16-byte pieces a thread stages
     __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * BP];
@@ -478,7 +509,23 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
         rt = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (FQ - 1) * 4, 0, 0));
         rd = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(dr, tid % FQ * 4, 0, 0));
     };
-    if (a.nchunk) fetch(back ? a.nchunk - 1 : 0, true);
+    // the state of chunk c (live = false: nowhere).  Issued behind the loads of
+    // the next chunk, which are waited for without it
+    auto put = [&](uint32_t c, bool live) {
+        const auto r = rsrc(slots + (size_t)c * (2 * FN * FP), live ? 2 * FN * FP * 2 : 0);
+        const uint32_t at = (state_at(w, n0 / 16, 0) + 16 * li + 4 * lq) * 2;
+#pragma unroll
+        for (int i = 0; i < NTL; ++i) {
+            floatx4 v = s[i];
+            const s4v hi = take4(v), lo = take4(v);
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, hi), r, at, state_at(0, i, 0) * 2, 0);
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, lo), r, at, state_at(0, i, 1) * 2, 0);
+        }
+    };
+    if (a.nchunk) {
+        fetch(back ? a.nchunk - 1 : 0, true);
+        put(back ? a.nchunk - 1 : 0, true);
+    }
     for (uint32_t k = 0; k < a.nchunk; ++k) {
         const uint32_t c = back ? a.nchunk - 1 - k : k;
         lds_barrier();
@@ -495,22 +542,13 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
         W[tid % FQ] = (back ? 1.0f : rd) * __expf(back ? rl : rt - rl);      // (both halves of the block the same)
         const float dq = __expf(rt);
         lds_barrier();
-        bf16* slot = slots + (size_t)c * (2 * FN * FP) + state_at(w, n0 / 16, 0) + 16 * li + 4 * lq;
 #pragma unroll
-        for (int i = 0; i < NTL; ++i) {
-            floatx4 v = s[i];
-            *reinterpret_cast<s4v*>(slot + state_at(0, i, 0)) = take4(v);
-            *reinterpret_cast<s4v*>(slot + state_at(0, i, 1)) = take4(v);
-            s[i] *= dq;
-        }
-        // the next chunk's loads are the youngest accesses: waiting for them
-        // at the top waits for nothing that was issued later
+        for (int i = 0; i < NTL; ++i) s[i] *= dq;
         fetch(back ? max(c, 1u) - 1 : min(c + 1, a.nchunk - 1), k + 1 < a.nchunk);
-        // the weighted rows in three pieces: the gradient of the first state is
-        // given in fp32
-        s8v f[FQ / 32][3];
-#pragma unroll
-        for (int ks = 0; ks < FQ / 32; ++ks) {
+        // The rows, weighted, in pieces: three backwards, as the gradient of the
+        // first state is given in fp32; two forwards, where the states are only
+        // kept as two.  A piece's products run while the next rows are split.
+        auto split = [&](int ks, s8v (&f)[3]) {
             // k = token in the order 4 q .. + 3, 16 + 4 q .. + 3 of each 32:
             // the transposing loads meet no bank twice
             const bf16* xp = Xs + (32 * ks + 4 * lq + tk) * FXP + 16 * w + 4 * tc;
@@ -525,18 +563,27 @@ template <int NC> __global__ __launch_bounds__(W_NT) void ssd_bwd_walk_bf16_kern
 #pragma unroll
             for (int e = 0; e < 3; ++e) {
                 const s4v lo = take4(v0);
-                f[ks][e] = cat8(lo, take4(v1));
+                f[e] = cat8(lo, take4(v1));
             }
-        }
+        };
+        auto products = [&](auto pieces) {
+            s8v f[2][3];
+            split(0, f[0]);
 #pragma unroll
-        for (int ks = 0; ks < FQ / 32; ++ks)
+            for (int ks = 0; ks < FQ / 32; ++ks) {
+                if (ks + 1 < FQ / 32) split(ks + 1, f[(ks + 1) % 2]);
 #pragma unroll
-            for (int i = 0; i < NTL; ++i) {
-                const bf16* bp = Bs + (32 * ks + 4 * lq + tk) * BP + 16 * i + 4 * tc;
-                const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 16 * BP));
+                for (int i = 0; i < NTL; ++i) {
+                    const bf16* bp = Bs + (32 * ks + 4 * lq + tk) * BP + 16 * i + 4 * tc;
+                    const s8v bt = cat8(ld_tr(bp), ld_tr(bp + 16 * BP));
 #pragma unroll
-                for (int e = 0; e < 3; ++e) s[i] = mma(f[ks][e], bt, s[i]);
+                    for (int e = 0; e < decltype(pieces)::value; ++e) s[i] = mma(f[ks % 2][e], bt, s[i]);
+                }
             }
+        };
+        if (back) products(std::integral_constant<int, 3>{});
+        else products(std::integral_constant<int, 2>{});
+        put(back ? max(c, 1u) - 1 : min(c + 1, a.nchunk - 1), k + 1 < a.nchunk);
     }
     if (back && a.d_state0)
 #pragma unroll
@@ -1101,7 +1148,7 @@ Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     p.share = (size_t)batch * d.L * d.n_groups * d.N;
     p.q = (size_t)p.nslice * batch * d.H * d.L;
     p.part = (size_t)batch * d.H * p.nslice * p.nchunk * 3;
-    p.steps = fast ? (size_t)batch * d.H * p.nchunk * FQ : 0;
+    p.steps = (size_t)batch * d.H * p.nchunk * (fast ? FQ : 1);
     // every array starts on a 16-byte address
     for (size_t* n : {&p.states, &p.share, &p.q, &p.part, &p.steps}) *n = (*n + 3) / 4 * 4;
     return p;
@@ -1112,7 +1159,8 @@ bool fast_dims(const lssm_ssd_dims& d, int act) {
 }
 
 template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArgs& a) {
-    ssd_bwd_walk_kernel<T, NT><<<dim3(a.H * a.nslice, a.batch, 2), G_NT, 0, s>>>(a);
+    if (a.nchunk) ssd_bwd_own_kernel<T, NT><<<dim3(a.H * a.nslice * 2, a.nchunk, a.batch), G_NT, 0, s>>>(a);
+    ssd_bwd_scan_kernel<<<dim3((a.P * a.N + G_NT - 1) / G_NT * 2, a.H, a.batch), G_NT, 0, s>>>(a);
     if (a.nchunk)
         ssd_bwd_chunk_kernel<T, NT><<<dim3(a.nchunk * a.nsplit * a.G, a.batch), G_NT, 0, s>>>(a);
 }
@@ -1150,11 +1198,7 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
         if (a.batch) {
             if (fast) {
                 if (a.nchunk) ssd_bwd_steps_kernel<<<dim3(a.nchunk, a.H, a.batch), FQ, 0, s>>>(a);
-                const char* ev = getenv("WALK_NC");
-                const int nc = ev ? atoi(ev) : 128;
-                if (nc == 128) ssd_bwd_walk_bf16_kernel<128><<<dim3(a.H * a.nslice, a.batch, 2), W_NT, 0, s>>>(a);
-                else if (nc == 64) ssd_bwd_walk_bf16_kernel<64><<<dim3(a.H * a.nslice * 2, a.batch, 2), W_NT, 0, s>>>(a);
-                else ssd_bwd_walk_bf16_kernel<32><<<dim3(a.H * a.nslice * 4, a.batch, 2), W_NT, 0, s>>>(a);
+                ssd_bwd_walk_bf16_kernel<<<dim3(a.H * a.nslice * (FN / NC), a.batch, 2), W_NT, 0, s>>>(a);
                 if (a.nchunk)
                     ssd_bwd_chunk_bf16_kernel<<<dim3(a.nchunk * a.nsplit * a.G, a.batch), F_NT, 0, s>>>(a);
             } else if (a.N <= 64) launch_generic<T, 64>(s, a);
