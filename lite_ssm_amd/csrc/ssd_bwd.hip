@@ -84,27 +84,51 @@ template <typename T> __device__ __forceinline__ Steps chunk_steps(const SsdBwdA
     return {s, __shfl(s, GQ - 1), dt};
 }
 
-// rows 0 .. rows - 1 of a [rows][stride] array, n columns, into LDS
-// [GQ][pitch] (pitch a multiple of four), zeros behind the ends (W columns in
-// all); 16 bytes at a time where the rows are whole and aligned
-template <typename T, int W> __device__ __forceinline__ void load_tile(float* dst, int pitch, const T* src, size_t stride,
-                                                                       uint32_t rows, uint32_t n) {
-    constexpr int E = 16 / sizeof(T);
-    if (n == W && (((uintptr_t)src | (stride * sizeof(T))) & 15) == 0) {
-        typedef T TE __attribute__((ext_vector_type(E)));
+// whether rows of n elements `stride` apart can be taken 16 bytes at a time
+template <typename T> __device__ __forceinline__ bool whole16(const T* src, size_t stride, uint32_t n) {
+    return n % (16 / sizeof(T)) == 0 && (((uintptr_t)src | (stride * sizeof(T))) & 15) == 0;
+}
+
+// A [rows <= GQ][n <= W] piece of an array of rows `stride` apart on its way
+// into LDS [GQ][pitch] as fp32, zeros behind the ends, by NTH threads: get()
+// loads 16 bytes at a time into registers, put() stores them.
+template <typename T, int W, int NTH> struct Tile {
+    static constexpr int E = 16 / sizeof(T), PER = W / E, ALL = GQ * PER, V = (ALL + NTH - 1) / NTH;
+    typedef T TE __attribute__((ext_vector_type(E)));
+    TE v[V];
+    __device__ __forceinline__ void get(const T* src, size_t stride, uint32_t rows, uint32_t n) {
 #pragma unroll
-        for (uint32_t k = 0; k < (GQ * W / E + G_NT - 1) / G_NT; ++k) {
-            const uint32_t i = threadIdx.x + k * G_NT, r = i / (W / E), c = i % (W / E) * E;
-            if (GQ * W / E % G_NT && i >= GQ * W / E) break;
-            TE v = TE(0);
-            if (r < rows) v = *reinterpret_cast<const TE*>(src + r * stride + c);
+        for (int k = 0; k < V; ++k) {
+            const uint32_t i = threadIdx.x + k * NTH, r = i / PER, c = i % PER * E;
+            v[k] = TE(0);
+            if (r < rows && c < n) v[k] = *reinterpret_cast<const TE*>(src + r * stride + c);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = TE(0);
+    }
+    __device__ __forceinline__ void put(float* dst, int pitch) const {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const uint32_t i = threadIdx.x + k * NTH, r = i / PER, c = i % PER * E;
+            if (ALL % NTH && i >= ALL) break;
 #pragma unroll
             for (int e = 0; e < E; e += 4)
-                *reinterpret_cast<floatx4*>(dst + r * pitch + c + e) = floatx4{to_f(v[e]), to_f(v[e + 1]), to_f(v[e + 2]), to_f(v[e + 3])};
+                *reinterpret_cast<floatx4*>(dst + r * pitch + c + e) =
+                    floatx4{to_f(v[k][e]), to_f(v[k][e + 1]), to_f(v[k][e + 2]), to_f(v[k][e + 3])};
         }
+    }
+};
+template <typename T, int W, int NTH> __device__ __forceinline__ void load_tile(float* dst, int pitch, const T* src,
+                                                                                size_t stride, uint32_t rows, uint32_t n) {
+    if (whole16(src, stride, n)) {
+        Tile<T, W, NTH> t;
+        t.get(src, stride, rows, n);
+        t.put(dst, pitch);
         return;
     }
-    for (uint32_t i = threadIdx.x; i < GQ * W; i += G_NT) {
+    for (uint32_t i = threadIdx.x; i < GQ * W; i += NTH) {
         const uint32_t r = i / W, c = i % W;
         dst[r * pitch + c] = (r < rows && c < n) ? to_f(src[r * stride + c]) : 0.0f;
     }
@@ -123,9 +147,9 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ow
     const uint32_t g = h / (a.H / a.G);
     const int tid = threadIdx.x, lane = tid % WAVE, li = lane % 16, lq = lane / 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    load_tile<T, GP>(Rs, GXP, (const T*)(back ? a.dY : a.X) + ((size_t)b * L + t0) * a.H * P + (size_t)h * P + p0,
+    load_tile<T, GP, G_NT>(Rs, GXP, (const T*)(back ? a.dY : a.X) + ((size_t)b * L + t0) * a.H * P + (size_t)h * P + p0,
                      (size_t)a.H * P, tl, pn);
-    load_tile<T, NT>(Cs, NP, (const T*)(back ? a.C : a.B) + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl,
+    load_tile<T, NT, G_NT>(Cs, NP, (const T*)(back ? a.C : a.B) + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl,
                      N);
     if (w == 0) {
         const Steps st = chunk_steps<T>(a, b, h, t0, tl);
@@ -185,85 +209,153 @@ __global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
 }
 
 // The chunks' gradients: block = chunk, sequence, group, share of the group's
-// (head, slice) pairs.  dB and dC of the share stay in registers.
-template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
-    constexpr int NP = NT + 4, TN = NT / 64;
-    __shared__ __attribute__((aligned(16))) float Bs[GQ * NP], Cs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
+// (head, slice) pairs.  dB and dC of the share stay in registers.  NW waves;
+// waves 0 .. 3 own the four tiles of S and M (tokens T0, J0) and of dx (tokens
+// T0, rows J0); eight waves split the k of dx over the state's columns.  The
+// next pair's rows and states are on their way into registers meanwhile, where
+// they can be taken 16 bytes at a time.  Two blocks fit a CU up to N = 128.
+template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
+    constexpr int NP = NT + 4, TN = NT / (16 * NW), NTH = 64 * NW, KG = NW / 4;
+    __shared__ __attribute__((aligned(16))) float Bs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
     __shared__ __attribute__((aligned(16))) float Xs[GQ * GXP], Ys[GQ * GXP], Ms[GQ * GXP];
+    __shared__ floatx4 part[KG > 1 ? 4 * WAVE : 1];
     __shared__ double Lc[GQ];
-    __shared__ float DT[GQ], EL[GQ], ER[GQ], RS[2][GQ], CS[2][GQ], VO[4][GQ], UO[2][GQ], red[4][2];
+    __shared__ float DT[GQ], EL[GQ], ER[GQ], SL[GQ], RS[2][GQ], CS[2][GQ], VO[NW][GQ], UO[2][GQ], red[NW][2];
     const uint32_t P = a.P, N = a.N, L = a.L, hpg = a.H / a.G;
     const uint32_t c = blockIdx.x % a.nchunk, sp = blockIdx.x / a.nchunk % a.nsplit;
     const uint32_t g = blockIdx.x / a.nchunk / a.nsplit, b = blockIdx.y;
     const uint32_t t0 = c * GQ, tl = min((uint32_t)GQ, L - t0);
     const int tid = threadIdx.x, lane = tid % WAVE, li = lane % 16, lq = lane / 16;
-    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const int T0 = w / 2, J0 = w % 2;      // this wave's tile of S, M (tokens) and of dx (tokens T0, rows J0)
+    const int w = __builtin_amdgcn_readfirstlane(tid / WAVE), kg = w / 4;
+    const int T0 = w % 4 / 2, J0 = w % 2;
 
-    load_tile<T, NT>(Bs, NP, (const T*)a.B + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl, N);
-    load_tile<T, NT>(Cs, NP, (const T*)a.C + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl, N);
+    // C B^T, and C where dC's products leave it; C is not needed between
+    const T* Cg = (const T*)a.C + ((size_t)b * L + t0) * a.G * N + (size_t)g * N;
+    load_tile<T, NT, NTH>(Bs, NP, (const T*)a.B + ((size_t)b * L + t0) * a.G * N + (size_t)g * N, (size_t)a.G * N, tl, N);
+    load_tile<T, NT, NTH>(Hs, NP, Cg, (size_t)a.G * N, tl, N);
     __syncthreads();
     floatx4 cb{0, 0, 0, 0};
     for (int k = 0; k < NT / 4; ++k)
-        cb = mma4(Cs[(16 * T0 + li) * NP + 4 * k + lq], Bs[(16 * J0 + li) * NP + 4 * k + lq], cb);
-
+        cb = mma4(Hs[(16 * T0 + li) * NP + 4 * k + lq], Bs[(16 * J0 + li) * NP + 4 * k + lq], cb);
+    floatx4 cr[2][TN];
     floatx4 dc[2][TN], db[2][TN], ssum{0, 0, 0, 0};
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int i = 0; i < TN; ++i) dc[q][i] = db[q][i] = floatx4{0, 0, 0, 0};
+        for (int i = 0; i < TN; ++i) {
+            dc[q][i] = db[q][i] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) cr[q][i][r] = Hs[(16 * q + 4 * lq + r) * NP + 16 * (w + NW * i) + li];
+        }
 
     const uint32_t pairs = hpg * a.nslice, per = (pairs + a.nsplit - 1) / a.nsplit;
-    for (uint32_t v = sp * per; v < min(pairs, (sp + 1) * per); ++v) {
-        const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice, p0 = sl * GP, pn = min((uint32_t)GP, P - p0);
-        const size_t row0 = ((size_t)b * L + t0) * a.H * P + (size_t)h * P + p0, hp = (size_t)a.H * P;
-        const size_t slot = (((size_t)b * a.H + h) * a.nchunk + c) * P * N + (size_t)p0 * N;
+    const uint32_t v_first = sp * per, v_end = min(pairs, v_first + per);
+    const size_t hp = (size_t)a.H * P;
+    Tile<T, GP, NTH> tx, ty;
+    Tile<float, NT, NTH> th, tg;
+    // (arrays and strides: the same answer for every pair)
+    const bool whole = whole16((const T*)a.X, hp, P) && whole16((const T*)a.dY, hp, P) && whole16(a.hst, N, N) && GP % (16 / sizeof(T)) == 0;
+    auto at = [&](uint32_t v, uint32_t& h, uint32_t& sl, size_t& row0, size_t& slot) {
+        h = g * hpg + v / a.nslice;
+        sl = v % a.nslice;
+        row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * GP;
+        slot = (((size_t)b * a.H + h) * a.nchunk + c) * P * N + (size_t)sl * GP * N;
+    };
+    auto fetch = [&](uint32_t v) {
+        uint32_t h, sl;
+        size_t row0, slot;
+        at(v, h, sl, row0, slot);
+        const uint32_t pn = min((uint32_t)GP, P - sl * GP);
+        tx.get((const T*)a.X + row0, hp, tl, pn);
+        ty.get((const T*)a.dY + row0, hp, tl, pn);
+        th.get(a.hst + slot, N, pn, N);
+        tg.get(a.gst + slot, N, pn, N);
+    };
+    if (whole && v_first < v_end) fetch(v_first);
+    for (uint32_t v = v_first; v < v_end; ++v) {
+        uint32_t h, sl;
+        size_t row0, slot;
+        at(v, h, sl, row0, slot);
+        const uint32_t p0 = sl * GP, pn = min((uint32_t)GP, P - p0);
         __syncthreads();
-        load_tile<T, GP>(Xs, GXP, (const T*)a.X + row0, hp, tl, pn);
-        load_tile<T, GP>(Ys, GXP, (const T*)a.dY + row0, hp, tl, pn);
-        load_tile<float, NT>(Hs, NP, a.hst + slot, N, pn, N);
-        load_tile<float, NT>(Gs, NP, a.gst + slot, N, pn, N);
-        double tot = 0.0;
-        if (w == 0) {
+        if (whole) {
+            tx.put(Xs, GXP);
+            ty.put(Ys, GXP);
+            th.put(Hs, NP);
+            tg.put(Gs, NP);
+        } else {
+            load_tile<T, GP, NTH>(Xs, GXP, (const T*)a.X + row0, hp, tl, pn);
+            load_tile<T, GP, NTH>(Ys, GXP, (const T*)a.dY + row0, hp, tl, pn);
+            load_tile<float, NT, NTH>(Hs, NP, a.hst + slot, N, pn, N);
+            load_tile<float, NT, NTH>(Gs, NP, a.gst + slot, N, pn, N);
+        }
+        if (w == NW - 1) {
             const Steps st = chunk_steps<T>(a, b, h, t0, tl);
-            tot = st.tot;
             if (lane < GQ) {
                 Lc[lane] = st.lc;
                 DT[lane] = st.dt;
                 EL[lane] = expf((float)st.lc);
                 ER[lane] = expf((float)(st.tot - st.lc));
+                SL[lane] = lane < (int)tl ? dt_slope<T>(a, b, t0 + lane, h) : 0.0f;
             }
         }
         __syncthreads();
-        // S and M of this wave's tile; row and column sums of K
-        floatx4 sd{0, 0, 0, 0};
-        if (T0 >= J0)
-            for (int k = 0; k < GP / 4; ++k)
-                sd = mma4(Ys[(16 * T0 + li) * GXP + 4 * k + lq], Xs[(16 * J0 + li) * GXP + 4 * k + lq], sd);
-        const int j = 16 * J0 + li;
-        float col = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = 16 * T0 + 4 * lq + r;
-            const float e = t >= j ? expf((float)(Lc[t] - Lc[j])) : 0.0f;
-            const float m = cb[r] * e, kk = sd[r] * m;
-            ssum[r] += sd[r] * e * DT[j];
-            Ms[t * GXP + j] = m;
-            const float row = group_sum<16>(kk * DT[j]);
-            if (li == 0) RS[J0][t] = row;
-            col += kk;
+        if (whole) {
+            if (v + 1 < v_end) {
+                fetch(v + 1);
+            } else {
+                // (not kept over the loop for this path's sake)
+                tx.clear();
+                ty.clear();
+                th.clear();
+                tg.clear();
+            }
         }
-        col += __shfl_xor(col, 16);
-        col += __shfl_xor(col, 32);
-        if (lq == 0) CS[T0][j] = col;
+        // S and M of this wave's tile; row and column sums of K
+        const int j = 16 * J0 + li;
+        if (kg == 0) {
+            floatx4 sd{0, 0, 0, 0};
+            if (T0 >= J0)
+                for (int k = 0; k < GP / 4; ++k)
+                    sd = mma4(Ys[(16 * T0 + li) * GXP + 4 * k + lq], Xs[(16 * J0 + li) * GXP + 4 * k + lq], sd);
+            float col = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = 16 * T0 + 4 * lq + r;
+                const float e = t >= j ? expf((float)(Lc[t] - Lc[j])) : 0.0f;
+                const float m = cb[r] * e, kk = sd[r] * m;
+                ssum[r] += sd[r] * e * DT[j];
+                Ms[t * GXP + j] = m;
+                const float row = group_sum<16>(kk * DT[j]);
+                if (li == 0) RS[J0][t] = row;
+                col += kk;
+            }
+            col += __shfl_xor(col, 16);
+            col += __shfl_xor(col, 32);
+            if (lq == 0) CS[T0][j] = col;
+        }
+        if (kg == KG - 1) {
+            // <G1, h0> and the sum of dy.x, by the last four waves
+            float gh = 0.0f, yx = 0.0f;
+            const int u = tid - 256 * (KG - 1);
+            for (int i = u; i < GP * NT; i += 256) gh += Hs[i / NT * NP + i % NT] * Gs[i / NT * NP + i % NT];
+            for (int i = u; i < GQ * GP; i += 256) yx += Xs[i / GP * GXP + i % GP] * Ys[i / GP * GXP + i % GP];
+            gh = wave_sum(gh);
+            yx = wave_sum(yx);
+            if (lane == 0) {
+                red[w % 4][0] = gh;
+                red[w % 4][1] = yx;
+            }
+        }
         // the parts that meet the states
         float vo[2][4] = {};
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const int n = 16 * (w + 4 * i) + li;
+                const int n = 16 * (w + NW * i) + li;
                 floatx4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
+#pragma unroll
                 for (int k = 0; k < GP / 4; ++k) {
                     x = mma4(Ys[(16 * q + li) * GXP + 4 * k + lq], Hs[(4 * k + lq) * NP + n], x);
                     y = mma4(Xs[(16 * q + li) * GXP + 4 * k + lq], Gs[(4 * k + lq) * NP + n], y);
@@ -273,7 +365,7 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
                     const int t = 16 * q + 4 * lq + r;
                     const float d = EL[t] * x[r];
                     dc[q][i][r] += d;
-                    vo[q][r] += d * Cs[t * NP + n];
+                    vo[q][r] += d * cr[q][i][r];
                     db[q][i][r] += DT[t] * ER[t] * y[r];
                 }
             }
@@ -285,53 +377,55 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
                 if (li == 0) VO[w][16 * q + 4 * lq + r] = s;
             }
         floatx4 dx{0, 0, 0, 0};
-        for (int k = 0; k < NT / 4; ++k)
-            dx = mma4(Bs[(16 * T0 + li) * NP + 4 * k + lq], Gs[(16 * J0 + li) * NP + 4 * k + lq], dx);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int t = 16 * T0 + 4 * lq + r;
-            dx[r] *= ER[t];
-            const float u = group_sum<16>(dx[r] * Xs[t * GXP + 16 * J0 + li]);
-            if (li == 0) UO[J0][t] = u;
+#pragma unroll 8
+        for (int k = 0; k < NT / 4 / KG; ++k) {
+            const int n = 4 * (k + kg * (NT / 4 / KG)) + lq;
+            dx = mma4(Bs[(16 * T0 + li) * NP + n], Gs[(16 * J0 + li) * NP + n], dx);
         }
-        float gh = 0.0f, yx = 0.0f;
-        for (int i = tid; i < GP * NT; i += G_NT) gh += Hs[i / NT * NP + i % NT] * Gs[i / NT * NP + i % NT];
-        for (int i = tid; i < GQ * GP; i += G_NT) yx += Xs[i / GP * GXP + i % GP] * Ys[i / GP * GXP + i % GP];
-        gh = wave_sum(gh);
-        yx = wave_sum(yx);
-        if (lane == 0) {
-            red[w][0] = gh;
-            red[w][1] = yx;
+        if (KG > 1 && kg == 1) part[(w % 4) * WAVE + lane] = dx;
+        __syncthreads();
+        if (kg == 0) {
+            if (KG > 1) dx += part[w * WAVE + lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = 16 * T0 + 4 * lq + r;
+                dx[r] *= ER[t];
+                const float u = group_sum<16>(dx[r] * Xs[t * GXP + 16 * J0 + li]);
+                if (li == 0) UO[J0][t] = u;
+            }
+#pragma unroll
+            for (int k = 0; k < GQ / 4; ++k)
+                dx = mma4(Ms[(4 * k + lq) * GXP + 16 * T0 + li], Ys[(4 * k + lq) * GXP + 16 * J0 + li], dx);
+            const float D = a.D ? to_f(((const T*)a.D)[h]) : 0.0f;
+            const uint32_t p = 16 * J0 + li;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t t = 16 * T0 + 4 * lq + r;
+                if (t < tl && p < pn) ((T*)a.dX)[row0 + t * hp + p] = from_f<T>(fmaf(DT[t], dx[r], D * Ys[t * GXP + p]));
+            }
         }
         __syncthreads();
-        for (int k = 0; k < GQ / 4; ++k)
-            dx = mma4(Ms[(4 * k + lq) * GXP + 16 * T0 + li], Ys[(4 * k + lq) * GXP + 16 * J0 + li], dx);
-        const float D = a.D ? to_f(((const T*)a.D)[h]) : 0.0f;
-        const uint32_t p = 16 * J0 + li;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t t = 16 * T0 + 4 * lq + r;
-            if (t < tl && p < pn) ((T*)a.dX)[row0 + t * hp + p] = from_f<T>(fmaf(DT[t], dx[r], D * Ys[t * GXP + p]));
-        }
         // a_t: pairs of a source before t and a sink from t on
-        if (w == 0) {
+        if (w == NW - 1) {
             const int t = min(lane, GQ - 1);
             const float dt = lane < GQ ? DT[t] : 0.0f, uo = UO[0][t] + UO[1][t], cs = CS[0][t] + CS[1][t];
-            float pre = lane < GQ ? dt * uo : 0.0f;
+            float pre = lane < GQ ? dt * uo : 0.0f, suf = RS[0][t] + RS[1][t] - dt * cs;
             const float own = pre;
-            float suf = lane < GQ ? (VO[0][t] + VO[1][t]) + (VO[2][t] + VO[3][t]) + (RS[0][t] + RS[1][t]) - dt * cs : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) suf += VO[i][t];
+            if (lane >= GQ) suf = 0.0f;
 #pragma unroll
             for (int d = 1; d < GQ; d <<= 1) {
                 const float x = __shfl_up(pre, d), y = __shfl_down(suf, d);
                 if (lane >= d) pre += x;
                 if (lane + d < GQ) suf += y;
             }
-            const float edge = expf((float)tot) * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
+            const float edge = EL[GQ - 1] * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
             const float da = edge + (pre - own) + suf;
             const float A = -expf(to_f(((const T*)a.A_log)[h]));
             float q = 0.0f;
             if (lane < (int)tl) {
-                q = (uo + cs + A * da) * dt_slope<T>(a, b, t0 + lane, h);
+                q = (uo + cs + A * da) * SL[t];
                 a.q[(((size_t)sl * a.batch + b) * a.H + h) * L + t0 + lane] = q;
             }
             const float dA = wave_sum(dt * da);
@@ -346,18 +440,20 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ch
     }
     // within the chunk: sum of S over the share's heads with B and C
     __syncthreads();
+    load_tile<T, NT, NTH>(Hs, NP, Cg, (size_t)a.G * N, tl, N);
+    if (kg == 0)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) Ms[(16 * T0 + 4 * lq + r) * GXP + 16 * J0 + li] = ssum[r];
+        for (int r = 0; r < 4; ++r) Ms[(16 * T0 + 4 * lq + r) * GXP + 16 * J0 + li] = ssum[r];
     __syncthreads();
     const size_t base = (size_t)sp * a.share;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int i = 0; i < TN; ++i) {
-            const uint32_t n = 16 * (w + 4 * i) + li;
+            const uint32_t n = 16 * (w + NW * i) + li;
             for (int k = 0; k < GQ / 4; ++k) {
                 dc[q][i] = mma4(Ms[(16 * q + li) * GXP + 4 * k + lq], Bs[(4 * k + lq) * NP + n], dc[q][i]);
-                db[q][i] = mma4(Ms[(4 * k + lq) * GXP + 16 * q + li], Cs[(4 * k + lq) * NP + n], db[q][i]);
+                db[q][i] = mma4(Ms[(4 * k + lq) * GXP + 16 * q + li], Hs[(4 * k + lq) * NP + n], db[q][i]);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -1162,7 +1258,7 @@ template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArg
     if (a.nchunk) ssd_bwd_own_kernel<T, NT><<<dim3(a.H * a.nslice * 2, a.nchunk, a.batch), G_NT, 0, s>>>(a);
     ssd_bwd_scan_kernel<<<dim3((a.P * a.N + G_NT - 1) / G_NT * 2, a.H, a.batch), G_NT, 0, s>>>(a);
     if (a.nchunk)
-        ssd_bwd_chunk_kernel<T, NT><<<dim3(a.nchunk * a.nsplit * a.G, a.batch), G_NT, 0, s>>>(a);
+        ssd_bwd_chunk_kernel<T, NT, NT == 64 ? 4 : 8><<<dim3(a.nchunk * a.nsplit * a.G, a.batch), NT == 64 ? 256 : 512, 0, s>>>(a);
 }
 
 }  // namespace
