@@ -96,10 +96,10 @@ template <typename T, int W, int NTH> struct Tile {
     static constexpr int E = 16 / sizeof(T), PER = W / E, ALL = GQ * PER, V = (ALL + NTH - 1) / NTH;
     typedef T TE __attribute__((ext_vector_type(E)));
     TE v[V];
-    __device__ __forceinline__ void get(const T* src, size_t stride, uint32_t rows, uint32_t n) {
+    __device__ __forceinline__ void get(uint32_t tid, const T* src, size_t stride, uint32_t rows, uint32_t n) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const uint32_t i = threadIdx.x + k * NTH, r = i / PER, c = i % PER * E;
+            const uint32_t i = tid + k * NTH, r = i / PER, c = i % PER * E;
             v[k] = TE(0);
             if (r < rows && c < n) v[k] = *reinterpret_cast<const TE*>(src + r * stride + c);
         }
@@ -108,10 +108,10 @@ template <typename T, int W, int NTH> struct Tile {
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] = TE(0);
     }
-    __device__ __forceinline__ void put(float* dst, int pitch) const {
+    __device__ __forceinline__ void put(uint32_t tid, float* dst, int pitch) const {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const uint32_t i = threadIdx.x + k * NTH, r = i / PER, c = i % PER * E;
+            const uint32_t i = tid + k * NTH, r = i / PER, c = i % PER * E;
             if (ALL % NTH && i >= ALL) break;
 #pragma unroll
             for (int e = 0; e < E; e += 4)
@@ -124,8 +124,8 @@ template <typename T, int W, int NTH> __device__ __forceinline__ void load_tile(
                                                                                 size_t stride, uint32_t rows, uint32_t n) {
     if (whole16(src, stride, n)) {
         Tile<T, W, NTH> t;
-        t.get(src, stride, rows, n);
-        t.put(dst, pitch);
+        t.get(threadIdx.x, src, stride, rows, n);
+        t.put(threadIdx.x, dst, pitch);
         return;
     }
     for (uint32_t i = threadIdx.x; i < GQ * W; i += NTH) {
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
 // T0, rows J0); eight waves split the k of dx over the state's columns.  The
 // next pair's rows and states are on their way into registers meanwhile, where
 // they can be taken 16 bytes at a time.  Two blocks fit a CU up to N = 128.
-template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
+template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW, NT == 256 ? 2 : 4) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
     constexpr int NP = NT + 4, TN = NT / (16 * NW), NTH = 64 * NW, KG = NW / 4;
     __shared__ __attribute__((aligned(16))) float Bs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
     __shared__ __attribute__((aligned(16))) float Xs[GQ * GXP], Ys[GQ * GXP], Ms[GQ * GXP];
@@ -225,7 +225,7 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW) void
     const uint32_t c = blockIdx.x % a.nchunk, sp = blockIdx.x / a.nchunk % a.nsplit;
     const uint32_t g = blockIdx.x / a.nchunk / a.nsplit, b = blockIdx.y;
     const uint32_t t0 = c * GQ, tl = min((uint32_t)GQ, L - t0);
-    const int tid = threadIdx.x, lane = tid % WAVE, li = lane % 16, lq = lane / 16;
+    int tid = threadIdx.x, lane = tid % WAVE, li = lane % 16, lq = lane / 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / WAVE), kg = w / 4;
     const int T0 = w % 4 / 2, J0 = w % 2;
 
@@ -266,10 +266,10 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW) void
         size_t row0, slot;
         at(v, h, sl, row0, slot);
         const uint32_t pn = min((uint32_t)GP, P - sl * GP);
-        tx.get((const T*)a.X + row0, hp, tl, pn);
-        ty.get((const T*)a.dY + row0, hp, tl, pn);
-        th.get(a.hst + slot, N, pn, N);
-        tg.get(a.gst + slot, N, pn, N);
+        tx.get(tid, (const T*)a.X + row0, hp, tl, pn);
+        ty.get(tid, (const T*)a.dY + row0, hp, tl, pn);
+        th.get(tid, a.hst + slot, N, pn, N);
+        tg.get(tid, a.gst + slot, N, pn, N);
     };
     if (whole && v_first < v_end) fetch(v_first);
     for (uint32_t v = v_first; v < v_end; ++v) {
@@ -277,12 +277,14 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW) void
         size_t row0, slot;
         at(v, h, sl, row0, slot);
         const uint32_t p0 = sl * GP, pn = min((uint32_t)GP, P - p0);
+        // (places are formed again for each pair instead of being kept)
+        asm volatile("" : "+v"(tid), "+v"(lane), "+v"(li), "+v"(lq));
         __syncthreads();
         if (whole) {
-            tx.put(Xs, GXP);
-            ty.put(Ys, GXP);
-            th.put(Hs, NP);
-            tg.put(Gs, NP);
+            tx.put(tid, Xs, GXP);
+            ty.put(tid, Ys, GXP);
+            th.put(tid, Hs, NP);
+            tg.put(tid, Gs, NP);
         } else {
             load_tile<T, GP, NTH>(Xs, GXP, (const T*)a.X + row0, hp, tl, pn);
             load_tile<T, GP, NTH>(Ys, GXP, (const T*)a.dY + row0, hp, tl, pn);
@@ -1156,6 +1158,7 @@ template <typename T> __global__ __launch_bounds__(R_NT) void ssd_bwd_finish_ker
         const size_t n = (size_t)a.batch * a.L * a.G * a.N, i = ((size_t)blk * R_NT + tid) * 4;
         if (i >= n) return;
         float x[4] = {}, y[4] = {};
+#pragma unroll 8
         for (uint32_t s = 0; s < a.nsplit; ++s) {
             const floatx4 u = *reinterpret_cast<const floatx4*>(a.bpart + s * a.share + i);
             const floatx4 v = *reinterpret_cast<const floatx4*>(a.cpart + s * a.share + i);
