@@ -100,6 +100,10 @@ template <int R> __device__ __forceinline__ void repack(u32x4 (&q)[R]) {
     for (int i = 0; i < R; ++i) asm volatile("" : "+v"(q[i]));
 }
 
+// Lane 0's sums for the whole wave: a multiplication may be folded into the
+// lanes' first addition, whose two sides then round differently.
+__device__ __forceinline__ Soft same(Soft a) { return {a.m, readlane_f(a.S, 0), readlane_f(a.T, 0)}; }
+
 // What a row gives in the end.
 struct RowOut { float max, ls, H; };
 __device__ __forceinline__ RowOut row_out(Soft a) {
@@ -248,6 +252,7 @@ __global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
     Soft b = moved({sm[l], sS[l], sT[l]}, M);
     b.S = group_sum<LP_NW>(b.S);
     b.T = group_sum<LP_NW>(b.T);
+    b = same(b);
     const RowOut o = row_out(b);
     if (tid == 0) {
         if (a.S == 1) {
@@ -378,6 +383,7 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
     s = moved(s, wave_max(s.m));
     s.S = wave_sum(s.S);
     s.T = wave_sum(s.T);
+    s = same(s);
     const RowOut o = row_out(s);
     if (tid == 0) {
         const int t = a.tokens ? a.tokens[r] : -1;

@@ -322,3 +322,22 @@ def test_captured_and_replayed(ctx, V, k):
         torch.cuda.synchronize()
         for a, b in zip((lp, H, st, ids, tl, d), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("V", [50280, 131072])
+def test_equal_logits_have_equal_log_probabilities(ctx, V):
+    """Many ties among the likeliest of many rows: equal logits get the same
+    bits, in the order of their ids, and a second call gives the same bits."""
+    M, k = 600, 20
+    x, t = logits(M, V, torch.bfloat16, 3)
+    x = (x * 4).round() / 4
+    code = L.BF16
+    a, b = call(ctx, x, t, k, code), call(ctx, x, t, k, code)
+    for n in a:
+        assert torch.equal(a[n], b[n]), n
+    v = x.cpu().gather(1, a["top_ids"].long())
+    lp = a["top_logprobs"]
+    same = v[:, 1:] == v[:, :-1]
+    assert bool(same.any())
+    assert torch.equal(lp[:, 1:] == lp[:, :-1], same)
+    assert bool((a["top_ids"][:, 1:] > a["top_ids"][:, :-1])[same].all())
