@@ -498,6 +498,18 @@ int lssm_engine_reset(lssm_engine* e);
  * `next_ids` (device int32 [batch]). */
 int lssm_engine_prefill(lssm_engine* e, const int32_t* ids, uint32_t batch, uint32_t L,
                         int32_t* next_ids);
+/* lssm_engine_prefill that also scores: after each of the batch * L positions,
+ * the log probability of tokens[b, l] as the next token (device int32 [batch, L];
+ * ids shifted by one score the sequence itself; negative: none), the entropy
+ * (or NULL) and the top_k likeliest tokens, as lssm_token_logprobs gives them from
+ * the positions' logits in the activation dtype.  tokens and logprob may be NULL
+ * together.  The lm_head runs over all positions, in blocks: the first call
+ * allocates a buffer for one (at most 128 MiB, or 128 rows).  No counterpart in
+ * the reference, which computes the last position's logits only
+ * (mamba2_block.cpp:296-315). */
+int lssm_engine_score(lssm_engine* e, const int32_t* ids, uint32_t batch, uint32_t L,
+                      int32_t* next_ids, const int32_t* tokens, float* logprob, float* entropy,
+                      int32_t* top_ids, float* top_logprobs, uint32_t top_k);
 /* One decode step for `batch` sequences: reads ids (device int32 [batch]),
  * writes logits and greedy next ids (device, may alias ids). */
 int lssm_engine_decode(lssm_engine* e, const int32_t* ids, uint32_t batch, int32_t* next_ids);

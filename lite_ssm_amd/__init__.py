@@ -176,6 +176,7 @@ _SIGS = {
     "lssm_engine_destroy": ([_vp], _i),
     "lssm_engine_reset": ([_vp], _i),
     "lssm_engine_prefill": ([_vp, _vp, _u32, _u32, _vp], _i),
+    "lssm_engine_score": ([_vp, _vp, _u32, _u32] + [_vp] * 6 + [_u32], _i),
     "lssm_engine_decode": ([_vp, _vp, _u32, _vp], _i),
     "lssm_engine_decode_graph": ([_vp, _vp, _u32, _vp, _u32], _i),
     "lssm_engine_logits": ([_vp, C.POINTER(_vp)], _i),

@@ -20,7 +20,7 @@ import sys
 CLI_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lssm_cli")
 # flags of lssm_cli that take a value (the others are switches)
 _VALUED = {"--model", "--tokenizer", "--tokens", "--top-p", "--temperature", "--seed", "--input-ids",
-           "--dump-logits", "--eos"}
+           "--dump-logits", "--eos", "--top-logprobs"}
 
 
 def split_args(argv):
@@ -63,6 +63,8 @@ def main(argv=None) -> int:
     if not ids:
         raise SystemExit("lite-ssm: empty prompt after tokenization")
     cmd = [CLI_PATH] + flags + ["--input-ids", ",".join(map(str, ids))]
+    if "--score" in flags:
+        return subprocess.run(cmd).returncode     # its lines name ids
     if not eos_set and sp.eos_id() >= 0:
         cmd += ["--eos", str(sp.eos_id())]
     r = subprocess.run(cmd, stdout=subprocess.PIPE)

@@ -14,6 +14,8 @@
 //     the ids and takes greedy ids there (the reference embeds and samples on
 //     the host, lite_ssm_cli.cpp:237-244, 296-303).  --top-p copies the logits
 //     to the host and samples there as the reference does.
+// --score (no counterpart in the reference) gives the prompt's own log
+// probabilities instead of generating.
 // Text prompts need SentencePiece, which this build does not link (the
 // reference fetches it at configure time); `python -m lite_ssm_amd.cli`
 // tokenizes with the sentencepiece Python module and runs this binary with
@@ -57,6 +59,8 @@ struct Args {
     bool eos_set = false;
     bool quiet = false;
     bool probe_only = false;
+    bool score = false;
+    uint32_t top_logprobs = 0;
 };
 
 // usage and input errors exit 2, library errors 1 (as the reference CLI)
@@ -79,6 +83,9 @@ void usage() {
                  "  --input-ids IDS     prompt token ids, comma or space separated\n"
                  "  --eos ID            stop after generating ID\n"
                  "  --dump-logits PATH  write the last step's logits as fp32\n"
+                 "  --score             print each prompt id's log probability given those before it\n"
+                 "                      (one \"ID LOGPROB\" line an id from the second on), generate nothing\n"
+                 "  --top-logprobs K    with --score: the K likeliest ids too, as ID:LOGPROB (up to 64)\n"
                  "  --probe-only        map the file, touch every page, report RSS\n"
                  "  --tokenizer PATH    accepted; text prompts go through python -m lite_ssm_amd.cli\n");
 }
@@ -117,6 +124,8 @@ Args parse_args(int argc, char** argv) {
         else if (k == "--eos") { a.eos_id = static_cast<uint32_t>(std::stoul(value("--eos"))); a.eos_set = true; }
         else if (k == "--quiet") a.quiet = true;
         else if (k == "--probe-only") a.probe_only = true;
+        else if (k == "--score") a.score = true;
+        else if (k == "--top-logprobs") a.top_logprobs = static_cast<uint32_t>(std::stoul(value("--top-logprobs")));
         else if (k == "-h" || k == "--help") { usage(); std::exit(0); }
         else if (!k.empty() && k[0] == '-') die("unknown flag: " + std::string(k));
         else words.emplace_back(k);
@@ -126,6 +135,9 @@ Args parse_args(int argc, char** argv) {
         die("provide a prompt text positionally, --input-ids, or --probe-only");
     }
     if (!a.input_ids.empty() && !words.empty()) die("can't combine --input-ids with a positional prompt");
+    if (a.top_logprobs && !a.score) die("--top-logprobs needs --score");
+    if (a.top_logprobs > LSSM_LOGPROB_MAX_TOP) die("--top-logprobs: at most " + std::to_string(LSSM_LOGPROB_MAX_TOP));
+    if (a.score && words.empty() && a.input_ids.size() < 2) die("--score needs at least two ids");
     for (size_t i = 0; i < words.size(); ++i) a.prompt_text += (i ? " " : "") + words[i];
     return a;
 }
@@ -248,6 +260,40 @@ int probe_only(const Args& args) {
     return 0;
 }
 
+// Log probabilities of the prompt's ids, from the second on, on stdout.
+void score(const Args& args, lssm_ctx* ctx, lssm_engine* eng, const int32_t* d_ids, int32_t* d_next, uint32_t vocab) {
+    const uint32_t L = static_cast<uint32_t>(args.input_ids.size()), K = std::min(args.top_logprobs, vocab);
+    std::vector<int32_t> next(args.input_ids.begin() + 1, args.input_ids.end());
+    next.push_back(-1);
+    // [tokens | logprob | entropy | top ids | top log p]
+    const size_t n = static_cast<size_t>(L) * (3 + 2 * static_cast<size_t>(K));
+    int32_t* d = nullptr;
+    check(lssm_malloc(reinterpret_cast<void**>(&d), 4 * n), "malloc");
+    check(lssm_memcpy_h2d(ctx, d, next.data(), 4 * static_cast<size_t>(L)), "copy tokens");
+    float* f = reinterpret_cast<float*>(d);
+    check(lssm_engine_reset(eng), "reset");
+    check(lssm_engine_score(eng, d_ids, 1, L, d_next, d, f + L, f + 2 * L, K ? d + 3 * L : nullptr,
+                            K ? f + static_cast<size_t>(3 + K) * L : nullptr, K),
+          "score");
+    std::vector<int32_t> raw(n);
+    check(lssm_memcpy_d2h(ctx, raw.data(), d, 4 * n), "copy log probabilities");
+    lssm_free(d);
+    std::vector<float> val(n);
+    std::memcpy(val.data(), raw.data(), 4 * n);
+    double sum = 0.0, entropy = 0.0;
+    for (uint32_t i = 0; i + 1 < L; ++i) {
+        sum += val[L + i];
+        entropy += val[2 * L + i];
+        std::printf("%d %.6f", next[i], val[L + i]);
+        for (uint32_t k = 0; k < K; ++k)
+            std::printf(" %d:%.6f", raw[3 * L + static_cast<size_t>(i) * K + k], val[static_cast<size_t>(3 + K) * L + static_cast<size_t>(i) * K + k]);
+        std::printf("\n");
+    }
+    std::fflush(stdout);
+    say(args.quiet, "[lite-ssm] score %u ids | log probability %.4f | perplexity %.4f | mean entropy %.4f", L - 1, sum,
+        std::exp(-sum / (L - 1)), entropy / (L - 1));
+}
+
 int generate(const Args& args) {
     using clk = std::chrono::steady_clock;
     if (!args.prompt_text.empty())
@@ -297,6 +343,15 @@ int generate(const Args& args) {
         }
     };
     int32_t* d_next = d_ids + L;
+    if (args.score) {
+        if (L < 2) die("--score needs at least two ids");
+        score(args, ctx, eng, d_ids, d_next, cfg.vocab_size);
+        lssm_free(d_ids);
+        lssm_engine_destroy(eng);
+        lssm_ctx_destroy(ctx);
+        lssm_ssm_close(f);
+        return 0;
+    }
     uint64_t rng = args.seed ? args.seed : 1u;
     // greedy: the engine's device argmax (first index of the maximum, the
     // reference's sample_greedy tie rule); top-p: sampled on the host

@@ -183,6 +183,53 @@ struct lssm_engine {
         return hipMemcpyAsync((char*)trace + (size_t)slot * n, h, n, hipMemcpyDeviceToDevice, st());
     }
 
+    // scoring (lssm_engine_score): the logits of a block of rows and the log
+    // probabilities' workspace, both allocated by the first call.  Blocks of 128
+    // MiB, which the GPU's last-level cache still holds when they are read back.
+    void* score_logits = nullptr;
+    void* score_ws = nullptr;
+    uint32_t score_rows = 0;
+    int score_alloc() {
+        if (score_logits) return LSSM_OK;
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        const hipError_t e = hipStreamIsCapturing(st(), &cap);
+        if (e != hipSuccess) return set_error(LSSM_EDEVICE, "engine_score: %s", hipGetErrorString(e));
+        LSSM_REQUIRE(cap == hipStreamCaptureStatusNone, "engine_score: the first call allocates and cannot be captured");
+        const uint32_t most = std::max<uint32_t>(128, (uint32_t)(((size_t)128 << 20) / ((size_t)vocab * es)) / 128 * 128);
+        const uint32_t rows = (uint32_t)std::min<uint64_t>((uint64_t)max_batch * max_seq, most);
+        void *l = nullptr, *w = nullptr;
+        if (int rc = alloc(&w, logprob_ws_bytes(rows, vocab, LSSM_LOGPROB_MAX_TOP))) return rc;
+        if (int rc = alloc(&l, (size_t)rows * vocab * es)) return rc;
+        score_ws = w;
+        score_rows = rows;
+        score_logits = l;
+        return LSSM_OK;
+    }
+    // The distributions after each of a prefill's R positions (hidden rows x):
+    // a, with its arrays for R rows.
+    hipError_t score(const void* x, uint32_t R, const LogprobArgs& all) const {
+        hipError_t e = hipSuccess;
+        for (uint32_t r = 0; r < R && e == hipSuccess; r += score_rows) {
+            const uint32_t n = std::min(score_rows, R - r);
+            e = launch_rmsnorm(st(), (const char*)x + (size_t)r * d_model * es, d_model, norm_f, normed, d_model, n, d_model,
+                               RMS_EPS, act);
+            if (e == hipSuccess)
+                e = linear(normed, d_model, lm_head, nullptr, score_logits, vocab, nullptr, n, vocab, d_model,
+                           LSSM_W_DENSE, LSSM_EPI_NONE);
+            LogprobArgs a = all;
+            a.x = score_logits;
+            a.stride = vocab;
+            a.rows = n;
+            a.tokens = a.tokens ? a.tokens + r : nullptr;
+            a.logprob = a.logprob ? a.logprob + r : nullptr;
+            a.entropy = a.entropy ? a.entropy + r : nullptr;
+            a.top_ids = a.top_ids ? a.top_ids + (size_t)r * a.K : nullptr;
+            a.top_logprobs = a.top_logprobs ? a.top_logprobs + (size_t)r * a.K : nullptr;
+            if (e == hipSuccess) e = launch_logprobs(st(), a, act, score_ws);
+        }
+        return e;
+    }
+
     // decode graphs of one step and of graph_unroll steps in a row (each
     // graph launch costs a gap of ~8 us before its first kernel; steps are
     // replayed unroll at a time, the rest one at a time).  2.7B batch 1: 1130
@@ -887,6 +934,39 @@ int lssm_engine_prefill(lssm_engine* e, const int32_t* ids, uint32_t batch, uint
     LSSM_REQUIRE(!e->trace || e->trace_bytes(L == 1 ? batch : batch * L) <= e->trace_cap,
                  "engine_prefill: trace buffer too small");
     return engine_finish(e, e->prefill(ids, batch, L, next_ids), "engine_prefill");
+}
+
+int lssm_engine_score(lssm_engine* e, const int32_t* ids, uint32_t batch, uint32_t L, int32_t* next_ids,
+                      const int32_t* tokens, float* logprob, float* entropy, int32_t* top_ids, float* top_logprobs,
+                      uint32_t top_k) {
+    if (int rc = check_engine(e)) return rc;
+    LSSM_REQUIRE(L >= 1 && L <= e->max_seq, "engine_score: L must be in [1, max_seq]");
+    LSSM_REQUIRE(batch >= 1 && batch <= e->max_batch, "engine_score: batch out of range");
+    LSSM_REQUIRE(ids && next_ids, "engine_score: null ids");
+    LSSM_REQUIRE((tokens != nullptr) == (logprob != nullptr), "engine_score: tokens and logprob go together");
+    LSSM_REQUIRE(top_k <= LSSM_LOGPROB_MAX_TOP && top_k <= e->vocab, "engine_score: top_k must be <= vocab and %d",
+                 LSSM_LOGPROB_MAX_TOP);
+    LSSM_REQUIRE(top_k == 0 || (top_ids && top_logprobs), "engine_score: top_k without top_ids and top_logprobs");
+    LSSM_REQUIRE(e->vocab <= LSSM_LOGPROB_MAX_VOCAB, "engine_score: vocab must be <= %d", LSSM_LOGPROB_MAX_VOCAB);
+    LSSM_REQUIRE((uint64_t)batch * L <= LSSM_LOGPROB_MAX_ROWS, "engine_score: too many positions");
+    for (const void* p : {(const void*)tokens, (const void*)logprob, (const void*)entropy, (const void*)top_ids,
+                          (const void*)top_logprobs})
+        LSSM_REQUIRE((uintptr_t)p % 4 == 0, "engine_score: arrays must be 4-byte aligned");
+    LSSM_REQUIRE(!e->trace || e->trace_bytes(L == 1 ? batch : batch * L) <= e->trace_cap,
+                 "engine_score: trace buffer too small");
+    if (int rc = e->score_alloc()) return rc;
+    LogprobArgs a{};
+    a.tokens = tokens;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_logprobs = top_logprobs;
+    a.V = e->vocab;
+    a.K = top_k;
+    a.status = e->ctx->status;
+    hipError_t err = e->prefill(ids, batch, L, next_ids);
+    if (err == hipSuccess) err = e->score(L == 1 ? e->d_hidden : e->hidden, batch * L, a);
+    return engine_finish(e, err, "engine_score");
 }
 
 int lssm_engine_decode(lssm_engine* e, const int32_t* ids, uint32_t batch, int32_t* next_ids) {

@@ -249,6 +249,17 @@ class Engine:
         B, L = ids.shape
         check(lib.lssm_engine_prefill(self.h, ids.data_ptr(), B, L, next_ids.data_ptr()))
 
+    def score(self, ids: torch.Tensor, next_ids: torch.Tensor, tokens=None, logprob=None, entropy=None,
+              top_ids=None, top_logprobs=None):
+        """Prefill that also gives, after each position of ids [B, L], the log
+        probability of tokens [B, L] (int32), the entropy [B, L] and the likeliest
+        tokens [B, L, k]; outputs that are None are left out."""
+        B, L = ids.shape
+        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        k = 0 if top_ids is None else top_ids.shape[-1]
+        check(lib.lssm_engine_score(self.h, ids.data_ptr(), B, L, next_ids.data_ptr(), p(tokens), p(logprob),
+                                    p(entropy), p(top_ids), p(top_logprobs), k))
+
     def decode(self, ids: torch.Tensor, next_ids: torch.Tensor):
         check(lib.lssm_engine_decode(self.h, ids.data_ptr(), ids.shape[0], next_ids.data_ptr()))
 
