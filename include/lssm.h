@@ -426,11 +426,12 @@ int lssm_argmax(lssm_ctx* ctx, const void* logits, int32_t* ids, uint32_t rows,
  * status word for that.
  * `ws`: at least lssm_token_logprobs_workspace bytes of device memory, 8-byte
  * aligned (0 bytes, NULL: rows short enough to need none); calls that may overlap need
- * one each.  vocab <= LSSM_LOGPROB_MAX_VOCAB, rows <= LSSM_LOGPROB_MAX_ROWS,
+ * one each.  Bytes for so many rows are enough for fewer.
+ * vocab <= LSSM_LOGPROB_MAX_VOCAB, rows * ceil(vocab / 32768) <= LSSM_LOGPROB_MAX_ROWS,
  * top_k <= LSSM_LOGPROB_MAX_TOP and vocab.  No counterpart in the reference, whose
  * sampler forms probabilities on the host (sampler.cpp). */
 #define LSSM_LOGPROB_MAX_VOCAB 2097152
-#define LSSM_LOGPROB_MAX_ROWS 16777215
+#define LSSM_LOGPROB_MAX_ROWS 2097151
 #define LSSM_LOGPROB_MAX_TOP 64
 uint64_t lssm_token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t top_k);
 int lssm_token_logprobs(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,

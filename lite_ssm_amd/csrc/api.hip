@@ -635,7 +635,9 @@ namespace {
 int logprob_checks(const LogprobArgs& a, int act, const char* name) {
     const size_t es = dtype_size(act);
     LSSM_REQUIRE(a.V >= 1 && a.V <= LSSM_LOGPROB_MAX_VOCAB, "%s: vocab must be in [1, %d]", name, LSSM_LOGPROB_MAX_VOCAB);
-    LSSM_REQUIRE(a.rows <= LSSM_LOGPROB_MAX_ROWS, "%s: rows must be <= %d", name, LSSM_LOGPROB_MAX_ROWS);
+    // (the threads of a launch count in 32 bits)
+    LSSM_REQUIRE((uint64_t)a.rows * ((a.V + 32767) / 32768) <= LSSM_LOGPROB_MAX_ROWS,
+                 "%s: rows must be <= %d, and that over the 32768ths of a row", name, LSSM_LOGPROB_MAX_ROWS);
     LSSM_REQUIRE(a.x, "%s: null logits", name);
     LSSM_REQUIRE(a.stride >= a.V && (!a.dx || a.dx_stride >= a.V), "%s: row stride smaller than the row", name);
     LSSM_REQUIRE((uintptr_t)a.x % es == 0 && (uintptr_t)a.dx % es == 0, "%s: logits not aligned to their type", name);

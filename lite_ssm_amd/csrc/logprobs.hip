@@ -29,11 +29,13 @@ namespace lssm {
 
 namespace {
 
-constexpr int LP_NT = 1024;                  // threads of a segment's block
-constexpr int LP_NW = LP_NT / WAVE;
-constexpr int LP_MAXR = 8;                   // 16-byte vectors a thread holds
+constexpr uint32_t LP_MAXR = 8;              // 16-byte vectors a thread holds
+constexpr uint32_t LP_WIDE = 1024, LP_SMALL = 256;   // threads of a segment's block
 constexpr int LP_CAP = 1024;                 // candidates of a segment's alternatives
-constexpr int LP_TAIL = LP_NT / 2;           // first thread of those that take a row's ragged end
+constexpr uint32_t LP_MAXS = 64;             // segments of a row
+constexpr int LP_JOIN = LSSM_LOGPROB_MAX_TOP * (LSSM_LOGPROB_MAX_TOP + 1) / 2;
+static_assert(LSSM_LOGPROB_MAX_VOCAB / 4 <= LP_MAXS * LP_WIDE * LP_MAXR, "segments");
+static_assert(LP_JOIN % 8 == 0 && LP_CAP % 8 == 0, "lists");
 constexpr float LOG2E = 1.44269504088896341f;
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -123,13 +125,22 @@ __device__ __forceinline__ void store_row(const LogprobArgs& a, uint32_t r, cons
 }
 
 // The K best of n unique keys in LDS: the rank of a key is the number of
-// larger ones, so the order in which they were collected does not show.
-template <int NT, typename F> __device__ __forceinline__ void rank_keys(const u64* keys, uint32_t n, uint32_t K, F put) {
-    for (uint32_t i = threadIdx.x; i < n; i += NT) {
-        const u64 k = keys[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += keys[j] > k ? 1u : 0u;
-        if (rank < K) put(rank, k);
+// larger ones, so the order in which they were collected does not show.  Four
+// lanes a key, each a quarter of the others (the list is filled up with zeros
+// to a multiple of 8, which are larger than none).
+template <int NT, typename F> __device__ __forceinline__ void rank_keys(u64* keys, uint32_t n, uint32_t K, F put) {
+    const uint32_t n8 = (n + 7) & ~7u, part = threadIdx.x % 4;
+    if (n + threadIdx.x < n8) keys[n + threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t i0 = 0; i0 < n; i0 += NT / 4) {
+        const uint32_t i = i0 + threadIdx.x / 4;
+        const u64 k = i < n ? keys[i] : ~0ull;
+        int rank = 0;
+#pragma unroll 4
+        for (uint32_t j = 2 * part; j < n8; j += 8) rank += (keys[j] > k ? 1 : 0) + (keys[j + 1] > k ? 1 : 0);
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xF, 0xF, false);
+        rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xF, 0xF, false);
+        if (part == 0 && i < n && (uint32_t)rank < K) put((uint32_t)rank, k);
     }
 }
 
@@ -157,11 +168,12 @@ template <typename T> struct RowSpan {
 
 // One segment of a row (the whole row where a.S == 1).
 // GRAD (a.S == 1, no alternatives): the gradient is written from the registers too.
-template <typename T, int R, bool GRAD>
-__global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
-    constexpr int E = Vec<T>::E;
+template <typename T, int R, bool GRAD, int LP_NT>
+__global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {
+    constexpr int E = Vec<T>::E, LP_NW = LP_NT / WAVE;
+    constexpr int LP_TAIL = LP_NT / 2;       // first thread of those that take a row's ragged end
     __shared__ float sm[LP_NW], sS[LP_NW], sT[LP_NW];
-    __shared__ uint32_t stau[LP_NW], scount;
+    __shared__ uint32_t stau[LP_NW], stau2[LP_NW], scount;
     __shared__ u64 keys[LP_CAP];
     __shared__ u64 swin[LP_NW];
     const uint32_t r = blockIdx.x / a.S, seg = blockIdx.x % a.S;
@@ -233,16 +245,23 @@ __global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
         sT[w] = s.T;
     }
     if (K) {
-        // the K-th best of the lanes' best values: at least K of the wave's
-        // values are no less, or tau is no more than the lowest finite one
-        // (which stands for lanes without a value).  Found bit by bit.
-        const uint32_t best = ord_of(m);
-        uint32_t tau = 0;
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t c = tau | (1u << bit);
+        // Two values that at least K of the block's are no less than: the K-th
+        // best of a wave's lanes' best values, and the lowest of the waves'
+        // ceil(K / waves)-th best ones.  Either may be the larger.  Found bit
+        // by bit, down to bits 12 (a 2^-11-th below them at most, which only
+        // lengthens the list).
+        constexpr uint32_t nw = LP_NW;
+        const uint32_t best = ord_of(m), K2 = (K + nw - 1) / nw;
+        uint32_t tau = 0, tau2 = 0;
+        for (int bit = 31; bit >= 12; --bit) {
+            const uint32_t c = tau | (1u << bit), c2 = tau2 | (1u << bit);
             if ((uint32_t)__popcll(__ballot(best >= c)) >= K) tau = c;
+            if ((uint32_t)__popcll(__ballot(best >= c2)) >= K2) tau2 = c2;
         }
-        if (tid % WAVE == 0) stau[w] = tau;
+        if (tid % WAVE == 0) {
+            stau[w] = tau;
+            stau2[w] = tau2;
+        }
         if (tid == 0) scount = 0;
     }
     __syncthreads();
@@ -265,28 +284,34 @@ __global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
         }
     }
     if (K) {
-        uint32_t tau = 1;
-        for (int i = 0; i < LP_NW; ++i) tau = max(tau, stau[i]);
+        uint32_t tau = ord_of(-FLT_MAX), tau2 = ~0u;
+#pragma unroll 4
+        for (int i = 0; i < LP_NW; ++i) {
+            tau = max(tau, stau[i]);
+            tau2 = min(tau2, stau2[i]);
+        }
+        tau = max(tau, tau2);
+        const float least = of_ord(tau);
         auto each = [&](auto f) {
             repack(q);
             uint32_t vb = v0 + tid;
             asm volatile("" : "+v"(vb));       // nor its places
-            if (ie < a.V) f(ord_of(xe), ie);
+            if (ie < a.V) f(xe, ie);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const uint32_t v = vb + i * LP_NT;
                 if (v < v1) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) f(ord_of(elem<T>(q[i], e)), sp.head + v * E + e);
+                    for (int e = 0; e < E; ++e) f(elem<T>(q[i], e), sp.head + v * E + e);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (ord_of(m) >= tau)
-            each([&](uint32_t ov, uint32_t idx) {
-                if (ov >= tau) {
+        if (m >= least)
+            each([&](float v, uint32_t idx) {
+                if (v >= least) {
                     const uint32_t at = atomicAdd(&scount, 1u);
-                    if (at < LP_CAP) keys[at] = key_of(ov, idx);
+                    if (at < LP_CAP) keys[at] = key_of(ord_of(v), idx);
                 }
             });
         __syncthreads();
@@ -310,7 +335,8 @@ __global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
             u64 last = ~0ull;
             for (uint32_t i = 0; i < K; ++i) {
                 u64 k = 0;
-                each([&](uint32_t ov, uint32_t idx) {
+                each([&](float v, uint32_t idx) {
+                    const uint32_t ov = ord_of(v);
                     const u64 c = ov ? key_of(ov, idx) : 0;
                     if (c < last && c > k) k = c;
                 });
@@ -370,7 +396,6 @@ __global__ __launch_bounds__(LP_NT) void logprob_seg_kernel(LogprobArgs a) {
 
 // Joins a row's segments: the sums, then the best of the segments' best.
 template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a) {
-    extern __shared__ u64 jkeys[];
     const uint32_t r = blockIdx.x, tid = threadIdx.x, S = a.S, K = a.K;
     const float* p = a.part + 3 * (size_t)r * S;
     Soft s{-FLT_MAX, 0.0f, 0.0f};
@@ -391,17 +416,39 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
         store_row(a, r, o, t >= 0 && (uint32_t)t < a.V ? to_f(row[t]) : 0.0f, t);
     }
     if (K == 0) return;
-    const uint32_t n = S * K;
-    for (uint32_t i = tid; i < n; i += 256) jkeys[i] = a.part_keys[(size_t)r * n + i];
+    // A segment's keys are in order: the i-th of the segment whose best has
+    // rank h among the segments' is behind i of its own and h others, so only
+    // those with h + i < K are looked at, K (K + 1) / 2 at most; and none
+    // below the lowest of all segments' ceil(K / S)-th keys.
+    __shared__ u64 keys[LP_JOIN];
+    __shared__ uint32_t rank[LP_MAXS], count, found;
+    const u64* in = a.part_keys + (size_t)r * S * K;
+    if (tid < S) {
+        keys[tid] = in[(size_t)tid * K];
+        keys[LP_MAXS + tid] = in[(size_t)tid * K + (K + S - 1) / S - 1];
+    }
+    if (tid == 0) count = found = 0;
     __syncthreads();
-    __shared__ uint32_t found;
-    if (tid == 0) found = 0;
+    if (tid < S) {
+        uint32_t h = 0;
+        for (uint32_t j = 0; j < S; ++j) h += keys[j] > keys[tid] ? 1u : 0u;
+        rank[tid] = h;
+    }
+    u64 least = ~0ull;
+    for (uint32_t j = 0; j < S; ++j) least = min(least, keys[LP_MAXS + j]);
     __syncthreads();
-    rank_keys<256>(jkeys, n, K, [&](uint32_t rank, u64 k) {
-        if (!k) return;                        // an empty place
+    for (uint32_t i = tid; i < S * K; i += 256) {
+        const uint32_t sg = i / K;
+        if (rank[sg] + (i - sg * K) < K) {
+            const u64 k = in[i];
+            if (k && k >= least) keys[atomicAdd(&count, 1u)] = k;      // 0: an empty place
+        }
+    }
+    __syncthreads();
+    rank_keys<256>(keys, count, K, [&](uint32_t place, u64 k) {
         atomicAdd(&found, 1u);
-        a.top_ids[(size_t)r * K + rank] = (int)~(uint32_t)k;
-        a.top_logprobs[(size_t)r * K + rank] = (of_ord((uint32_t)(k >> 32)) - o.max) - o.ls;
+        a.top_ids[(size_t)r * K + place] = (int)~(uint32_t)k;
+        a.top_logprobs[(size_t)r * K + place] = (of_ord((uint32_t)(k >> 32)) - o.max) - o.ls;
     });
     __syncthreads();
     for (uint32_t i = found + tid; i < K; i += 256) {
@@ -474,29 +521,52 @@ template <typename F> hipError_t with_type(int act, F f) {
 
 }  // namespace
 
-// Segments of a row.
-uint32_t logprob_segments(uint32_t rows, uint32_t vocab, int act) {
-    (void)rows;
-    const uint32_t e = act == LSSM_F32 ? 4u : 8u;
-    return std::max(1u, (vocab / e + LP_NT * LP_MAXR - 1) / (LP_NT * LP_MAXR));
+// How a row is cut: segments, threads a block, 16-byte vectors a thread.
+// Blocks of LP_WIDE threads, a segment as long as their registers hold; where
+// these are fewer than LP_FEW, blocks of LP_SMALL threads, as many as LP_WANT
+// allows (us, wide -> small, bf16, alternatives): 1 x 50280, 5: 11.5 -> 9.3;
+// 8 x 50280, 5: 12.4 -> 9.8; 1 x 256000, 20: 16.6 -> 14.8; 32 x 50280, 20:
+// 12.4 both; 64 x 50280, none: 7.2 -> 8.4; 128 x 50280, 5: 11.9 -> 14.3.
+// LP_WANT 256 and 1024 measured alike.
+constexpr uint32_t LP_FEW = 32, LP_WANT = 512;
+struct LogprobPlan { uint32_t S, nt, R; };
+static LogprobPlan plan_of(uint32_t rows, uint32_t vocab, int act) {
+    const uint32_t nv = std::max(1u, vocab / (act == LSSM_F32 ? 4u : 8u));
+    auto segs = [&](uint32_t nt, uint32_t R) { return (nv + nt * R - 1) / (nt * R); };
+    const uint32_t S = segs(LP_WIDE, LP_MAXR);
+    if ((uint64_t)rows * S < LP_FEW && segs(LP_SMALL, LP_MAXR) <= LP_MAXS) {
+        uint32_t R = 2;
+        while (R < LP_MAXR && (rows * segs(LP_SMALL, R) > LP_WANT || segs(LP_SMALL, R) > LP_MAXS)) R *= 2;
+        return {segs(LP_SMALL, R), LP_SMALL, R};
+    }
+    const uint32_t per = (nv + S - 1) / S;
+    return {S, LP_WIDE, per <= 2 * LP_WIDE ? 2u : per <= 4 * LP_WIDE ? 4u : 8u};
 }
+
+uint32_t logprob_segments(uint32_t rows, uint32_t vocab, int act) { return plan_of(rows, vocab, act).S; }
 
 // [part: 3 floats a segment, to a multiple of 8 bytes][keys: K a segment]
 static size_t part_bytes(uint32_t rows, uint32_t segs) { return ((size_t)rows * segs * 12 + 7) / 8 * 8; }
 
+// (of either type size, and enough for fewer rows too, which are cut finer)
 size_t logprob_ws_bytes(uint32_t rows, uint32_t vocab, uint32_t top_k) {
-    size_t n = 0;     // of either type size
-    for (int act : {LSSM_BF16, LSSM_F32}) {
-        const uint32_t S = logprob_segments(rows, vocab, act);
-        if (S > 1) n = std::max(n, part_bytes(rows, S) + (size_t)rows * S * top_k * 8);
-    }
+    size_t n = 0;
+    auto of = [&](uint32_t r) {
+        for (int act : {LSSM_BF16, LSSM_F32}) {
+            const uint32_t S = plan_of(r, vocab, act).S;
+            if (S > 1) n = std::max(n, part_bytes(r, S) + (size_t)r * S * top_k * 8);
+        }
+    };
+    for (uint32_t r = 1; r < std::min(rows, LP_FEW); ++r) of(r);
+    of(rows);
     return n;
 }
 
 hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws) {
-    a.S = logprob_segments(a.rows, a.V, act);
-    const uint32_t nv = a.V / (act == LSSM_F32 ? 4u : 8u);
-    a.seg_vecs = std::max(1u, (nv + a.S - 1) / a.S);
+    const LogprobPlan p = plan_of(a.rows, a.V, act);
+    const uint32_t nv = std::max(1u, a.V / (act == LSSM_F32 ? 4u : 8u));
+    a.S = p.S;
+    a.seg_vecs = (nv + p.S - 1) / p.S;
     if (a.S > 1) {
         a.part = static_cast<float*>(ws);
         a.part_keys = reinterpret_cast<unsigned long long*>(static_cast<char*>(ws) + part_bytes(a.rows, a.S));
@@ -507,13 +577,14 @@ hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws) {
         const bool grad = a.dx && a.S == 1;
         auto go = [&](auto rc) {
             constexpr int R = decltype(rc)::value;
-            if (grad) logprob_seg_kernel<T, R, true><<<grid, LP_NT, 0, s>>>(a);
-            else logprob_seg_kernel<T, R, false><<<grid, LP_NT, 0, s>>>(a);
+            if (p.nt == LP_SMALL && !grad) logprob_seg_kernel<T, R, false, LP_SMALL><<<grid, LP_SMALL, 0, s>>>(a);
+            else if (grad) logprob_seg_kernel<T, R, true, LP_WIDE><<<grid, LP_WIDE, 0, s>>>(a);
+            else logprob_seg_kernel<T, R, false, LP_WIDE><<<grid, LP_WIDE, 0, s>>>(a);
         };
-        if (a.seg_vecs <= 2 * LP_NT) go(std::integral_constant<int, 2>{});
-        else if (a.seg_vecs <= 4 * LP_NT) go(std::integral_constant<int, 4>{});
+        if (p.R == 2) go(std::integral_constant<int, 2>{});
+        else if (p.R == 4) go(std::integral_constant<int, 4>{});
         else go(std::integral_constant<int, 8>{});
-        if (a.S > 1) logprob_join_kernel<T><<<a.rows, 256, (size_t)a.S * a.K * 8, s>>>(a);
+        if (a.S > 1) logprob_join_kernel<T><<<a.rows, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !a.dx || grad) return e;
         return launch_logprobs_grad(s, a, act);

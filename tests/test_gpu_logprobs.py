@@ -341,3 +341,35 @@ def test_equal_logits_have_equal_log_probabilities(ctx, V):
     assert bool(same.any())
     assert torch.equal(lp[:, 1:] == lp[:, :-1], same)
     assert bool((a["top_ids"][:, 1:] > a["top_ids"][:, :-1])[same].all())
+
+
+@pytest.mark.parametrize("M", [1, 5, 40])
+@pytest.mark.parametrize("V", [4097, 50281, 140000])
+@pytest.mark.parametrize("how", ["ascending", "descending", "one value", "one wave", "alternating"])
+def test_alternatives_of_uneven_rows(ctx, M, V, how):
+    """Where the best logits lie together, or are all alike, and as many
+    alternatives as a row gives."""
+    i = torch.arange(V, device="cuda", dtype=torch.float32)
+    x = {"ascending": i / V, "descending": -i / V, "one value": 0 * i + 1,
+         "one wave": torch.where((i >= 512) & (i < 600), 5 + (i % 7), -i / V),
+         "alternating": torch.where(i % 2 == 0, 1.0, -1.0)}[how].repeat(M, 1)
+    t = torch.arange(M, dtype=torch.int32, device="cuda")
+    got = call(ctx, x, t, 64, L.F32)
+    ids = torch.sort(x[0].cpu(), descending=True, stable=True).indices[:64].int()
+    assert all(torch.equal(got["top_ids"][r], ids) for r in range(M))
+    lp = torch.log_softmax(x[0].double(), -1).cpu()[ids.long()]
+    bound = 28 * U + 2 * U * lp.abs()
+    for r in range(M):
+        close(got["top_logprobs"][r], lp, bound, "top_logprobs")
+
+
+@pytest.mark.parametrize("V,k", [(50280, 20), (256000, 5)])
+def test_a_workspace_for_many_rows_serves_fewer(ctx, V, k):
+    x, t = logits(40, V, torch.bfloat16, 5)
+    ws = torch.empty(ctx.token_logprobs_workspace(40, V, k), dtype=torch.uint8, device="cuda")
+    for M in (40, 31, 4, 1):
+        lp, ids = torch.empty(M, device="cuda"), torch.empty(M, k, dtype=torch.int32, device="cuda")
+        ctx.token_logprobs(x[:M], t[:M], lp, None, None, ids, torch.empty(M, k, device="cuda"), M, V, k, L.BF16, ws)
+        want = exact(x[:M], t[:M], k)
+        close(lp.cpu(), want[0], 28 * U + 2 * U * want[0].abs(), "logprob")
+        assert torch.equal(ids.cpu().long(), want[3])

@@ -28,6 +28,8 @@ def fwd(logits=P, stride=0, tokens=P, lp=P, H=P, st=P, ids=None, tl=None, rows=4
     (dict(V=0), "vocab must be"),
     (dict(V=2097153), "vocab must be"),
     (dict(rows=1 << 24), "rows must be"),
+    (dict(rows=1 << 21), "rows must be"),
+    (dict(rows=1 << 20, V=32769), "rows must be"),
     (dict(stride=99), "row stride"),
     (dict(logits=P + 1), "not aligned"),
     (dict(logits=P + 2, act=L.F32), "not aligned"),
@@ -82,8 +84,14 @@ def test_no_rows_is_nothing_to_do():
 
 def test_workspace_grows_with_what_it_holds():
     f = L.lib.lssm_token_logprobs_workspace
-    assert f(8, 100, 5) == 0 and f(8, 32768, 64) == 0
+    assert f(8, 100, 5) == 0 and f(800, 2048, 64) == 0
     one, more = f(1, 256000, 0), f(1, 256000, 20)
     assert 0 < one < more
-    assert f(700, 256000, 20) >= 700 * more - 8 * 700
     assert f(1, 2097153, 0) == 0 and f(1, 100, 65) == 0
+
+
+@pytest.mark.parametrize("k", [0, 5, 64])
+@pytest.mark.parametrize("V", [100, 2049, 50280, 65544, 256000, 2097152])
+def test_workspace_of_some_rows_is_enough_for_fewer(V, k):
+    sizes = [L.lib.lssm_token_logprobs_workspace(r, V, k) for r in range(1, 80)]
+    assert sizes == sorted(sizes)
