@@ -322,6 +322,7 @@ int ssd_bwd_checks(uint32_t batch, const lssm_ssd_dims& d, lssm_dtype act, const
     LSSM_REQUIRE(batch <= 65535, "%s: batch must be <= 65535", name);
     LSSM_REQUIRE(d.P <= 1024 && d.H <= 65535 && d.L <= LSSM_SSD_BWD_MAX_L, "%s: P must be <= 1024, H <= 65535, L <= %d", name,
                  LSSM_SSD_BWD_MAX_L);
+    LSSM_REQUIRE(ssd_bwd_launches(batch, d, act), "%s: batch * L * n_groups is too large", name);
     return LSSM_OK;
 }
 
@@ -354,6 +355,22 @@ int lssm_ssd_chunked_bwd(lssm_ctx* ctx, const void* X, const void* B, const void
     const size_t need = ssd_bwd_ws_bytes(batch, d, act);
     LSSM_REQUIRE(need == 0 || (ws && ws_bytes >= need), "%s: the workspace needs %zu bytes", name, need);
     LSSM_REQUIRE((uintptr_t)ws % 16 == 0, "%s: the workspace must be 16-byte aligned", name);
+    // what is read may not be written before the last launch that reads it
+    const size_t tok = (size_t)batch * d.L, hd = (size_t)d.H * es, x = tok * d.P * hd, bc = tok * d.n_groups * d.N * es,
+                 st = (size_t)batch * d.H * d.P * d.N * 4;
+    struct Range { const void* p; size_t n; };
+    const Range in[] = {{X, x}, {B, bc}, {C, bc}, {dt_raw, tok * hd}, {dt_bias, hd}, {A_log, hd}, {d.has_D ? D_skip : nullptr, hd},
+                        {state, st}, {dY, x}, {d_state, st}, {ws, need}};
+    const Range out[] = {{dX, x}, {dB, bc}, {dC, bc}, {d_dt, tok * hd}, {d_dt_bias, hd}, {dA_log, hd},
+                         {d.has_D ? dD : nullptr, hd}, {d_state0, st}};
+    auto apart = [](const Range& u, const Range& v) {
+        const uintptr_t a = (uintptr_t)u.p, b = (uintptr_t)v.p;
+        return !u.p || !v.p || a + u.n <= b || b + v.n <= a;
+    };
+    for (const Range& o : out) {
+        for (const Range& i : in) LSSM_REQUIRE(apart(o, i), "%s: an output overlaps an input or the workspace", name);
+        for (const Range& i : out) LSSM_REQUIRE(&i == &o || apart(o, i), "%s: outputs overlap", name);
+    }
     SsdBwdArgs a{};
     a.X = X;
     a.B = B;

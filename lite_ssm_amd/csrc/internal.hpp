@@ -180,10 +180,12 @@ struct SsdBwdArgs {
     float *bpart, *cpart;   // [share][batch][L][G][N], `share` floats a share
     float* q;               // [slice][batch][H][L]: gradient of dt_raw
     float* part;            // [batch][H][slice][chunk][3]: sums of d_dt_bias, dA_log and dD
-    float *lc, *dtv, *slope;   // bf16 form: [batch][H][chunk][token]: sums of A dt, dt, d dt / d raw
+    float *lc, *dtv, *slope, *w_fwd, *w_back;   // bf16 form: [batch][H][chunk][token]: sums of -A dt (fixed point), dt, d dt / d raw,
+                                // weights of the states; else lc: [batch][H][chunk], a chunk's decay
     size_t share;
     uint32_t row_blocks, dt_blocks;
 };
+bool ssd_bwd_launches(uint32_t batch, const lssm_ssd_dims& d, int act);   // false: too large for a launch
 size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act);
 hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, int act, void* ws);
 

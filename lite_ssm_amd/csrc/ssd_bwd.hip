@@ -22,7 +22,9 @@
 //         + sum_{s >= t > j} K[s, j],
 //   u_j = dt_j e^{Lq - Lc_j} x_j.(G1 B_j),  v_s = e^{Lc_s} C_s.(h0^T dy_s),
 //   K[s, j] = (dy_s.x_j)(C_s.B_j) E dt_j
-// which adds terms of one chunk only: no sum over the whole sequence cancels.
+// which adds terms of one chunk only, and only terms that the step's own decay is
+// part of: none is formed as a difference of longer sums, so a step that forgets
+// what came before it (A dt far below 0) keeps its gradient's digits.
 //
 // Three steps: the states h0 (forwards) and G1 (backwards) of every chunk are
 // kept; the chunks' gradients, in parallel; sums over heads, slices and chunks.
@@ -49,6 +51,12 @@ __device__ __forceinline__ floatx4 mma4(float a, float b, floatx4 c) {
 // The sums of A dt are held in 64 bits: differences of sums that grow along a
 // chunk are what every decay is the exponential of.
 // ---------------------------------------------------------------------------
+// A step's A dt below this is taken as this: e^-104 is 0 in fp32 and so is every
+// decay over such a step, and the sums behind it stay small enough to hold the
+// steps that follow.  (A NaN stays one.)
+constexpr double LEAST_STEP = -104.0;
+__device__ __forceinline__ double bounded(double x) { return x < LEAST_STEP ? LEAST_STEP : x; }
+
 constexpr int GQ = 32;      // tokens a chunk
 constexpr int GP = 32;      // state rows a slice
 constexpr int GXP = 36;     // LDS pitch of a [token][row] tile (= 4 modulo 64 banks x 9)
@@ -75,13 +83,31 @@ template <typename T> __device__ __forceinline__ Steps chunk_steps(const SsdBwdA
         dt = v > 20.0f ? v : log1pf(expf(v));
         dt = fminf(fmaxf(dt, a.dt_min), a.dt_max);
     }
-    double s = (double)A * (double)dt;
+    double s = bounded((double)A * (double)dt);
 #pragma unroll
     for (int d = 1; d < GQ; d <<= 1) {
         const double o = __shfl_up(s, d);
         if ((int)t >= d) s += o;
     }
     return {s, __shfl(s, GQ - 1), dt};
+}
+
+// The sums of a 16 x 16 tile's columns from each row on (the tile as its
+// product leaves it: rows 4 q .. 4 q + 3 of column i), `carry` behind its last
+// row; carry becomes the sum of all.
+__device__ __forceinline__ void from_row(floatx4& v, float& carry) {
+    v[2] += v[3];
+    v[1] += v[2];
+    v[0] += v[1];
+    const uint32_t q = threadIdx.x / 16 % 4;
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[0]), false, false);
+    const float odd = __uint_as_float(p[1]), both = __uint_as_float(p[0]) + odd;
+    const auto o = __builtin_amdgcn_permlane32_swap(__float_as_uint(both), __float_as_uint(both), false, false);
+    const float high = __uint_as_float(o[1]);
+    const float after = carry + ((q % 2 ? 0.0f : odd) + (q < 2 ? high : 0.0f));
+    carry += __uint_as_float(o[0]) + high;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += after;
 }
 
 // whether rows of n elements `stride` apart can be taken 16 bytes at a time
@@ -320,7 +346,8 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW, NT =
             if (T0 >= J0)
                 for (int k = 0; k < GP / 4; ++k)
                     sd = mma4(Ys[(16 * T0 + li) * GXP + 4 * k + lq], Xs[(16 * J0 + li) * GXP + 4 * k + lq], sd);
-            float col = 0.0f;
+            float col = 0.0f, below = 0.0f;
+            floatx4 kt;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int t = 16 * T0 + 4 * lq + r;
@@ -328,9 +355,16 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW, NT =
                 const float m = cb[r] * e, kk = sd[r] * m;
                 ssum[r] += sd[r] * e * DT[j];
                 Ms[t * GXP + j] = m;
-                const float row = group_sum<16>(kk * DT[j]);
-                if (li == 0) RS[J0][t] = row;
+                kt[r] = t > j ? kk * DT[j] : 0.0f;
                 col += kk;
+            }
+            // sinks from t on, sources of this tile before t
+            from_row(kt, below);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int t = 16 * T0 + 4 * lq + r;
+                const float row = group_sum<16>(t > j ? kt[r] : 0.0f);
+                if (li == 0) RS[J0][t] = row;
             }
             col += __shfl_xor(col, 16);
             col += __shfl_xor(col, 32);
@@ -411,19 +445,28 @@ template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW, NT =
         if (w == NW - 1) {
             const int t = min(lane, GQ - 1);
             const float dt = lane < GQ ? DT[t] : 0.0f, uo = UO[0][t] + UO[1][t], cs = CS[0][t] + CS[1][t];
-            float pre = lane < GQ ? dt * uo : 0.0f, suf = RS[0][t] + RS[1][t] - dt * cs;
-            const float own = pre;
+            // sources before t with the sinks behind the chunk, and, for t in its
+            // first half, with those of the second; sinks from t on with the
+            // sources before the chunk
+            float pre = lane < GQ ? dt * uo : 0.0f, half = lane < 15 ? dt * CS[1][t] : 0.0f, suf = 0.0f;
+            if (lane < GQ)
 #pragma unroll
-            for (int i = 0; i < NW; ++i) suf += VO[i][t];
-            if (lane >= GQ) suf = 0.0f;
+                for (int i = 0; i < NW; ++i) suf += VO[i][t];
 #pragma unroll
             for (int d = 1; d < GQ; d <<= 1) {
-                const float x = __shfl_up(pre, d), y = __shfl_down(suf, d);
-                if (lane >= d) pre += x;
+                const float x = __shfl_up(pre, d), y = __shfl_down(suf, d), z = __shfl_up(half, d);
+                if (lane >= d) {
+                    pre += x;
+                    half += z;
+                }
                 if (lane + d < GQ) suf += y;
             }
+            pre = __shfl_up(pre, 1);
+            half = __shfl_up(half, 1);
+            if (lane == 0) pre = 0.0f;
+            if (lane == 0 || lane >= 16) half = 0.0f;
             const float edge = EL[GQ - 1] * ((red[0][0] + red[1][0]) + (red[2][0] + red[3][0]));
-            const float da = edge + (pre - own) + suf;
+            const float da = (edge + pre) + (suf + ((RS[0][t] + RS[1][t]) + half));
             const float A = -expf(to_f(((const T*)a.A_log)[h]));
             float q = 0.0f;
             if (lane < (int)tl) {
@@ -523,8 +566,24 @@ __device__ __forceinline__ s4v take4(floatx4& v) {
     return __builtin_bit_cast(s4v, u32x2{a, b});
 }
 
-// dt and the sums of A dt of every chunk, zeros and the last sum behind the
-// end: block (chunk, head, sequence), a thread a token
+// The sums of A dt in the bf16 form: -Lc in units of 2^-18 (at most 128 104 2^18
+// < 2^32).  A decay's exponent is a difference of two, exact, each rounded by
+// 2^-19 whatever the sums have grown to (an fp32 sum passes that at 64); what
+// they decay is written in 16 bits.  The states' weights are formed from the
+// sums themselves.
+constexpr float LC_UNIT = 1.0f / 262144.0f;
+constexpr uint32_t LC_NAN = ~0u;
+__device__ __forceinline__ uint32_t to_units(double lc) { return lc == lc ? (uint32_t)(-lc * 262144.0 + 0.5) : LC_NAN; }
+// e^(Lc_t - Lc_j), t at or behind j
+__device__ __forceinline__ float decay_of(uint32_t t, uint32_t j) {
+    return __builtin_amdgcn_exp2f((float)(t - j) * (-LC_UNIT * 1.44269504088896341f));
+}
+// NaN for the sum up to a step behind a NaN one (A_log may be NaN)
+__device__ __forceinline__ float nan_of(uint32_t lc) { return lc == LC_NAN ? NAN : 0.0f; }
+
+// dt, the sums of A dt of every chunk and the walks' weights (from the sums in 64
+// bits), zeros and the last sum behind the end: block (chunk, head, sequence), a
+// thread a token
 __global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
     __shared__ double s[FQ];
     const uint32_t c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
@@ -535,7 +594,7 @@ __global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
         dt = v > 20.0f ? v : log1pf(expf(v));
         dt = fminf(fmaxf(dt, a.dt_min), a.dt_max);
     }
-    s[t] = A * (double)dt;
+    s[t] = bounded(A * (double)dt);
     __syncthreads();
     for (int d = 1; d < FQ; d <<= 1) {
         const double o = (int)t >= d ? s[t - d] : 0.0;
@@ -544,7 +603,9 @@ __global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
         __syncthreads();
     }
     const size_t at = (((size_t)b * a.H + h) * a.nchunk + c) * FQ + t;
-    a.lc[at] = (float)s[t];
+    reinterpret_cast<uint32_t*>(a.lc)[at] = to_units(s[t]);
+    a.w_back[at] = expf((float)s[t]);
+    a.w_fwd[at] = dt * expf((float)(s[FQ - 1] - s[t]));
     a.dtv[at] = dt;
     a.slope[at] = c * FQ + t < a.L ? dt_slope<bf16>(a, b, c * FQ + t, h) : 0.0f;
 }
@@ -576,8 +637,8 @@ __global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
     bf16* slots = (bf16*)(back ? a.gst : a.hst) + (((size_t)b * a.H + h) * a.nslice + sl) * a.nchunk * (2 * FN * FP);
     const bf16* rows = (const bf16*)(back ? a.dY : a.X) + (size_t)b * L * a.H * P + (size_t)h * P + sl * FP;
     const bf16* cols = (const bf16*)(back ? a.C : a.B) + (size_t)b * L * a.G * FN + (size_t)g * FN + n0;
-    const float* lc = a.lc + ((size_t)b * a.H + h) * a.nchunk * FQ;
-    const float* dtv = a.dtv + ((size_t)b * a.H + h) * a.nchunk * FQ;
+    const float* weights = (back ? a.w_back : a.w_fwd) + ((size_t)b * a.H + h) * a.nchunk * FQ;
+    const float* decays = a.w_back + ((size_t)b * a.H + h) * a.nchunk * FQ + FQ - 1;
     const size_t plain = (((size_t)b * a.H + h) * P + sl * FP + 16 * w + 4 * lq) * FN + n0 + li;
 
     floatx4 s[NTL];
@@ -587,7 +648,7 @@ __global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
         for (int r = 0; r < 4; ++r) s[i][r] = init ? init[plain + r * FN + 16 * i] : 0.0f;
 
     u32x4 rx[XV], rb[BV];
-    float rl = 0.0f, rt = 0.0f, rd = 0.0f;
+    float rw = 0.0f, rq = 0.0f;
     // the chunk's rows (behind the sequence's end, and for live = false: zeros,
     // as out of the resource's range)
     const uint32_t xat = tid / (FP / 8) * (a.H * P * 2) + tid % (FP / 8) * 16;
@@ -596,16 +657,15 @@ __global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
         const uint32_t t0 = c * FQ, tl = min((uint32_t)FQ, L - t0);
         const auto xr = rsrc(rows + (size_t)t0 * a.H * P, live ? ((tl - 1) * a.H * P + FP) * 2 : 0);
         const auto br = rsrc(cols + (size_t)t0 * a.G * FN, live ? ((tl - 1) * a.G * FN + NC) * 2 : 0);
-        const auto lr = rsrc(lc + t0, live ? FQ * 4 : 0), dr = rsrc(dtv + t0, live ? FQ * 4 : 0);
+        const auto wr = rsrc(weights + t0, live ? FQ * 4 : 0), qr = rsrc(decays + t0, live ? 4 : 0);
 #pragma unroll
         for (int i = 0; i < XV; ++i)
             rx[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, xat, i * (W_NT / (FP / 8)) * a.H * P * 2, 0);
 #pragma unroll
         for (int i = 0; i < BV; ++i)
             rb[i] = __builtin_amdgcn_raw_buffer_load_b128(br, bat, i * (W_NT / (NC / 8)) * a.G * FN * 2, 0);
-        rl = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, tid % FQ * 4, 0, 0));
-        rt = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(lr, (FQ - 1) * 4, 0, 0));
-        rd = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(dr, tid % FQ * 4, 0, 0));
+        rw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(wr, tid % FQ * 4, 0, 0));
+        rq = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(qr, 0, 0, 0));
     };
     // the state of chunk c (live = false: nowhere).  Issued behind the loads of
     // the next chunk, which are waited for without it
@@ -637,8 +697,8 @@ __global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
             const uint32_t j = tid + i * W_NT;
             *reinterpret_cast<u32x4*>(Bs + j / (NC / 8) * BP + j % (NC / 8) * 8) = rb[i];
         }
-        W[tid % FQ] = (back ? 1.0f : rd) * __expf(back ? rl : rt - rl);      // (both halves of the block the same)
-        const float dq = __expf(rt);
+        W[tid % FQ] = rw;      // (both halves of the block the same)
+        const float dq = rq;
         lds_barrier();
 #pragma unroll
         for (int i = 0; i < NTL; ++i) s[i] *= dq;
@@ -718,8 +778,9 @@ __device__ __forceinline__ float row_sums4(const floatx4& v) {
 __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) {
     __shared__ __attribute__((aligned(16))) bf16 stage[4 * FQ * FXP];
     __shared__ __attribute__((aligned(16))) floatx4 SS[F_TILES * WAVE], CB[F_TILES * WAVE];
-    __shared__ __attribute__((aligned(16))) float LC[FQ], DT[FQ], EL[FQ], ER[FQ], WB[FQ], AF[FQ];
-    __shared__ float SL[FQ], VO[8][FQ], RS[8][FQ], UO[FQ], CS[FQ], red[8][2];
+    __shared__ __attribute__((aligned(16))) float DT[FQ], EL[FQ], ER[FQ], WB[FQ], AF[FQ];
+    __shared__ __attribute__((aligned(16))) uint32_t LC[FQ];
+    __shared__ float SL[FQ], VO[8][FQ], RS[8][FQ], UO[FQ], CS[FQ], red[8][2], TL[6][FQ], TE[2];
     bf16 *Xs = stage, *Ys = stage + FQ * FXP, *Gh = stage + 2 * FQ * FXP, *Gl = stage + 3 * FQ * FXP;
     const uint32_t P = a.P, L = a.L, hpg = a.H / a.G;
     uint32_t tid = threadIdx.x;
@@ -736,8 +797,8 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     const uint32_t pairs = hpg * a.nslice, per = (pairs + a.nsplit - 1) / a.nsplit;
     const uint32_t v_first = sp * per, v_end = min(pairs, v_first + per);
     u32x4 rx[2], ry[2], rg[4], rh[4];
-    float rl = 0.0f, rt = 0.0f, rr = 0.0f, rd = 0.0f, rs = 0.0f;
-    uint32_t ra = 0, rD = 0;
+    float rd = 0.0f, rs = 0.0f;
+    uint32_t rl = 0, rt = 0, rr = 0, ra = 0, rD = 0;
     auto fetch = [&](uint32_t v, bool live) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
         const size_t row0 = ((size_t)b * L + t0) * hp + (size_t)h * P + sl * FP;
@@ -762,12 +823,12 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         const size_t sp0 = (((size_t)b * a.H + h) * a.nchunk + c) * FQ;
         const uint32_t some = live ? FQ * 4 : 0, tt = tid % FQ;
         const auto lr = rsrc(a.lc + sp0, some), dr = rsrc(a.dtv + sp0, some), sr = rsrc(a.slope + sp0, some);
-        auto one = [](auto r, uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * at, 0, 0)); };
+        auto one = [](auto r, uint32_t at) -> uint32_t { return __builtin_amdgcn_raw_buffer_load_b32(r, 4 * at, 0, 0); };
         rl = one(lr, tt);
         rt = one(lr, FQ - 1);
         rr = one(lr, tt >= 16 ? tt / 16 * 16 - 1 : 0);      // (token blocks past the first)
-        rd = one(dr, tt);
-        rs = one(sr, tt);
+        rd = __uint_as_float(one(dr, tt));
+        rs = __uint_as_float(one(sr, tt));
         ra = __builtin_amdgcn_raw_buffer_load_b16(rsrc((const bf16*)a.A_log + h, 2), 0, 0, 0);
         rD = __builtin_amdgcn_raw_buffer_load_b16(rsrc((const bf16*)a.D + h, a.D ? 2 : 0), 0, 0, 0);
     };
@@ -836,37 +897,55 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
     // 2 l and 2 l + 1.  The wave with the fewest tiles gathers a pair's sums and
     // finishes them while the others work on the next.
     constexpr int TAIL = 4;
-    float pre[2], suf[2], dir[2], tdt[2], tsl[2], tedge = 0.0f, tdd = 0.0f, tA = 0.0f;
+    float tA = 0.0f;
     auto gather = [&]() {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int t = 2 * lane + k;
-            float s = 0.0f;
+            float suf = 0.0f, in = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += VO[i][t];
+            for (int i = 0; i < 8; ++i) suf += VO[i][t];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += RS[i][t];
-            const float dt = DT[t], u = UO[t], cs = CS[t];
-            tsl[k] = SL[t];
-            tdt[k] = dt;
-            dir[k] = u + cs;
-            pre[k] = dt * u;
-            suf[k] = s - dt * cs;
+            for (int i = 0; i < 8; ++i) in += RS[i][t];
+            const float dt = DT[t], u = UO[t];
+            TL[0][t] = dt * u;
+            TL[1][t] = suf;
+            TL[2][t] = in;
+            TL[3][t] = u + CS[t];
+            TL[4][t] = dt;
+            TL[5][t] = SL[t];
         }
-        tedge = tdd = 0.0f;
+        float tedge = 0.0f, tdd = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             tedge += red[i][0];
             tdd += red[i][1];
         }
-        tedge *= EL[FQ - 1];
+        if (lane < 2) TE[lane] = lane ? tdd : tedge * EL[FQ - 1];
     };
     auto finish = [&](uint32_t v) {
         const uint32_t h = g * hpg + v / a.nslice, sl = v % a.nslice;
-        const float both = pre[0] + pre[1], own = suf[0] + suf[1];
-        const float p_in = tedge + (wave_prefix_sum(both) - both);
-        const float s_from = wave_sum(own) - wave_prefix_sum(own);      // behind this lane's
-        const float da0 = p_in + (s_from + own), da1 = (p_in + pre[0]) + (s_from + suf[1]);
+        float pre[2], suf[2], in[2], dir[2], tdt[2], tsl[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int t = 2 * lane + k;
+            pre[k] = TL[0][t];
+            suf[k] = TL[1][t];
+            in[k] = TL[2][t];
+            dir[k] = TL[3][t];
+            tdt[k] = TL[4][t];
+            tsl[k] = TL[5][t];
+        }
+        const float tedge = TE[0], tdd = TE[1];
+        // sums before and behind this lane's tokens (not as differences of
+        // longer ones: a step that forgets leaves far less than there was)
+        float before = __shfl_up(wave_prefix_sum(pre[0] + pre[1]), 1);
+        if (lane == 0) before = 0.0f;
+        float behind = __shfl(wave_prefix_sum(__shfl(suf[0] + suf[1], 63 - lane)), 62 - lane);
+        if (lane == 63) behind = 0.0f;
+        before += tedge;
+        behind += suf[1];
+        const float da0 = before + ((behind + suf[0]) + in[0]), da1 = (before + pre[0]) + (behind + in[1]);
         const float q0 = fmaf(tA, da0, dir[0]) * tsl[0], q1 = fmaf(tA, da1, dir[1]) * tsl[1];
         float* q = a.q + (((size_t)sl * a.batch + b) * a.H + h) * L + t0;
         if (2 * lane < (int)tl) q[2 * lane] = q0;
@@ -902,13 +981,13 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         }
         const float D = val((short)rD), A_h = -__expf(val((short)ra));
         if (tid < FQ) {
-            const float er = __expf(rt - rl);
+            const float er = decay_of(rt, rl) + nan_of(rt);
             LC[tid] = rl;
             DT[tid] = rd;
-            EL[tid] = __expf(rl);
+            EL[tid] = decay_of(rl, 0) + nan_of(rl);
             ER[tid] = er;
             WB[tid] = rd * er;
-            AF[tid] = __expf(rl - rr);
+            AF[tid] = decay_of(rl, rr);
             SL[tid] = rs;
         }
         lds_barrier();
@@ -963,7 +1042,8 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                 dx[p] = mma(cat8(ld_tr(Gh + at), ld_tr(Gh + at + 16 * FXP)), bf[ks], dx[p]);
                 dx[p] = mma(cat8(ld_tr(Gl + at), ld_tr(Gl + at + 16 * FXP)), bf[ks], dx[p]);
             }
-        const float erj = ER[j], dtj = DT[j], lcj = LC[j];
+        const float erj = ER[j], dtj = DT[j];
+        const uint32_t lcj = LC[j];
         float uo = 0.0f;
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
@@ -979,12 +1059,12 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
         // sinks T: dC^T [n][sink] of all sources before the chunk; S and M of column J
         const s8v xj0 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 8 * lq);
         const s8v xj1 = *reinterpret_cast<const s8v*>(Xs + j * FXP + 32 + 8 * lq);
-        float col = 0.0f, diag = 0.0f;
+        float col = 0.0f, diag = 0.0f, below = 0.0f;
 #pragma unroll
-        for (int T2 = 0; T2 < 8; T2 += 2) {
+        for (int T2 = 6; T2 >= 0; T2 -= 2) {
             s4v mh[2], ml[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 1; k >= 0; --k) {
                 const int T = T2 + k;
                 const bf16* yp = Ys + (16 * T + li) * FXP + 8 * lq;
                 const s8v y0 = *reinterpret_cast<const s8v*>(yp), y1 = *reinterpret_cast<const s8v*>(yp + 32);
@@ -1010,13 +1090,13 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                     const int id = tile_of(T, 0) + J;
                     floatx4 e;
                     if (T > J) {
-                        const float f = __expf(LC[16 * T - 1] - lcj);
+                        const float f = decay_of(LC[16 * T - 1], lcj);
                         e = *reinterpret_cast<const floatx4*>(AF + 16 * T + 4 * lq) * f;
                     } else {
-                        const floatx4 lt = *reinterpret_cast<const floatx4*>(LC + 16 * T + 4 * lq);
+                        const u32x4 lt = *reinterpret_cast<const u32x4*>(LC + 16 * T + 4 * lq);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            e[r] = 4 * lq + r >= li ? __expf(lt[r] - lcj) : 0.0f;
+                            e[r] = 4 * lq + r >= li ? decay_of(lt[r], lcj) : 0.0f;
                             diag += 4 * lq + r == li ? sd[r] : 0.0f;
                         }
                     }
@@ -1031,6 +1111,14 @@ __global__ __launch_bounds__(F_NT) void ssd_bwd_chunk_bf16_kernel(SsdBwdArgs a) 
                         row[r] = sdt * cb[r];
                     }
                     SS[id * WAVE + lane] = ss;
+                    // sinks from t on, this wave's sources before t
+                    if (T == J)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) row[r] = 4 * lq + r > li ? row[r] : 0.0f;
+                    from_row(row, below);
+                    if (T == J)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) row[r] = 4 * lq + r > li ? row[r] : 0.0f;
                     const float rsum = row_sums4(row);
                     if (li < 4) RS[w][16 * T + 4 * lq + li] = rsum;
                     mh[k] = take4(m);
@@ -1216,12 +1304,12 @@ template <typename F> hipError_t with_type(int act, F f) {
     return f(float{});
 }
 
-// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts][3 x steps]
+// The plan and the workspace: [h0 states][G1 states][dB parts][dC parts][q][head parts][5 x steps]
 struct Plan {
     bool fast;
     uint32_t nchunk, nslice, nsplit;
     size_t states, share, q, part, steps;      // floats of one of each
-    size_t floats() const { return 2 * states + 2 * nsplit * share + q + part + 3 * steps; }
+    size_t floats() const { return 2 * states + 2 * nsplit * share + q + part + 5 * steps; }
 };
 Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     Plan p;
@@ -1252,6 +1340,12 @@ Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     for (size_t* n : {&p.states, &p.share, &p.q, &p.part, &p.steps}) *n = (*n + 3) / 4 * 4;
     return p;
 }
+// (the threads of a launch's x count in 32 bits)
+bool launches(uint32_t batch, const lssm_ssd_dims& d, const Plan& p) {
+    const uint64_t rows = (p.share + 4 * R_NT - 1) / (4 * R_NT);
+    const uint64_t dts = (uint64_t)batch * ((d.L + R_T - 1) / R_T) * ((d.H + R_H - 1) / R_H);
+    return (uint64_t)p.nchunk * p.nsplit * d.n_groups * F_NT < (1ull << 32) && (rows + dts + d.H) * R_NT < (1ull << 32);
+}
 // (a chunk's rows within 32-bit byte offsets)
 bool fast_dims(const lssm_ssd_dims& d, int act) {
     return act == LSSM_BF16 && d.N == FN && d.P % FP == 0 && (uint64_t)d.H * std::max(d.P, d.N) * FQ * 2 < (1u << 31);
@@ -1265,6 +1359,10 @@ template <typename T, int NT> void launch_generic(hipStream_t s, const SsdBwdArg
 }
 
 }  // namespace
+
+bool ssd_bwd_launches(uint32_t batch, const lssm_ssd_dims& d, int act) {
+    return launches(batch, d, plan_of(batch, d, false)) && (!fast_dims(d, act) || launches(batch, d, plan_of(batch, d, true)));
+}
 
 // (the larger of both plans: alignment of the arrays decides at the call)
 size_t ssd_bwd_ws_bytes(uint32_t batch, const lssm_ssd_dims& d, int act) {
@@ -1289,6 +1387,8 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
     a.lc = a.part + p.part;
     a.dtv = a.lc + p.steps;
     a.slope = a.dtv + p.steps;
+    a.w_fwd = a.slope + p.steps;
+    a.w_back = a.w_fwd + p.steps;
     a.share = p.share;
     a.row_blocks = (uint32_t)((p.share + 4 * R_NT - 1) / (4 * R_NT));
     a.dt_blocks = a.batch * ((a.L + R_T - 1) / R_T) * ((a.H + R_H - 1) / R_H);

@@ -9,7 +9,7 @@ def forward(v, dt_min, dt_max):
     """Y and the final state; v: X, B, C, dt, dt_bias, A_log, D, state (64 bits)."""
     b, L, H, P = v["X"].shape
     hpg = H // v["B"].shape[2]
-    soft = torch.nn.functional.softplus(v["dt"] + v["dt_bias"], threshold=1e9)
+    soft = torch.logaddexp(v["dt"] + v["dt_bias"], torch.zeros((), dtype=torch.float64))
     dt, A = soft.clamp(dt_min, dt_max), -torch.exp(v["A_log"])
     h, ys = v["state"], []
     for t in range(L):
@@ -24,7 +24,7 @@ def grads(v, dt_min, dt_max, absolute=False):
     every sum added with a positive sign."""
     v = {k: t.double().cpu() for k, t in v.items()}
     raw = v["dt"] + v["dt_bias"]
-    soft = torch.nn.functional.softplus(raw, threshold=1e9)
+    soft = torch.logaddexp(raw, torch.zeros((), dtype=torch.float64))
     dt, A = soft.clamp(dt_min, dt_max), -torch.exp(v["A_log"])
     slope = torch.sigmoid(raw) * ((soft >= dt_min) & (soft <= dt_max))
     if absolute:

@@ -116,6 +116,41 @@ def test_slow_fast_and_clamped_steps(ctx, act, dt_scale):
     check(call(ctx, v, code, lo=1e-3, hi=5.0), v, dt, lo=1e-3, hi=5.0)
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("big", [30.0, 1000.0])
+def test_steps_that_forget_everything(ctx, act, big):
+    """Some steps as large as softplus gives them (no upper clamp), ordinary ones
+    behind them: a chunk's sums of A dt pass 10^5, and the decays of the ordinary
+    steps are as exact as before."""
+    code, dt = ACT[act]
+    v = inputs(dt, 2, 300, 4, 64, 2, 128, 41)
+    g = torch.Generator().manual_seed(42)
+    v["dt"] = torch.where(torch.rand(2, 300, 4, generator=g) < 0.3, torch.tensor(big, dtype=dt), v["dt"])
+    check(call(ctx, v, code, lo=0.0, hi=float("inf")), v, dt, lo=0.0, hi=float("inf"))
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_a_head_that_is_nan(ctx, act):
+    """Its gradients are NaN, and its group's dB and dC; the other group's are not touched."""
+    code, dt = ACT[act]
+    v = inputs(dt, 1, 200, 4, 64, 2, 128, 43)
+    v["A_log"][1] = float("nan")
+    got = call(ctx, v, code)
+    assert bool(got["dX"][:, :-1, 1].isnan().all()) and bool(got["dC"][:, 1:, 0].isnan().all())
+    assert bool(got["dB"][:, :-1, 0].isnan().all()) and bool(got["d_state0"][:, 1].isnan().all())
+    for k in ("dX", "d_dt"):
+        got[k][:, :, 1] = 0
+    for k in ("dB", "dC"):
+        got[k][:, :, 0] = 0
+    for k in ("d_dt_bias", "dA_log", "dD"):
+        got[k][1] = 0
+    got["d_state0"][:, 1] = 0
+    assert all(bool(x.isfinite().all()) for x in got.values())
+    v["A_log"][1] = 0
+    want = call(ctx, v, code)
+    assert torch.equal(got["dX"][:, :, 2:], want["dX"][:, :, 2:]) and torch.equal(got["dB"][:, :, 1], want["dB"][:, :, 1])
+
+
 @pytest.mark.parametrize("act", ["f32", "bf16"])
 def test_nothing_to_scan(ctx, act):
     """No tokens: the state's gradient passes through, parameters have none.

@@ -64,9 +64,31 @@ def call(ctx=CTX, batch=1, dims=None, act=L.BF16, ws=P, n=1 << 40, **over):
     (dict(ws=None), "workspace needs"),
     (dict(n=100), "workspace needs"),
     (dict(ws=P + 8), "16-byte aligned"),
+    (dict(dims=dict(L=1048576, H=256, G=256, P=1, N=1)), "too large"),
+    (dict(), "overlaps an input"),
 ])
 def test_refuses(kw, text):
     assert call(**kw) == 1
+    assert text in L.lib.lssm_last_error().decode()
+
+
+@pytest.mark.parametrize("where,text", [
+    (dict(dX="X"), "overlaps an input"),
+    (dict(d_state0="state"), "overlaps an input"),
+    (dict(dB="dY"), "overlaps an input"),
+    (dict(dA_log="A_log"), "overlaps an input"),
+    (dict(dC="dB"), "outputs overlap"),
+    (dict(d_dt="ws"), "the workspace"),
+])
+def test_refuses_what_overlaps(where, text):
+    names = ["X", "B", "C", "dt", "dt_bias", "A_log", "D", "state", "dY", "d_state", "dX", "dB", "dC", "d_dt", "d_dt_bias",
+             "dA_log", "dD", "d_state0", "ws"]
+    at = {k: P + (i << 16) for i, k in enumerate(names)}
+    over = dict(at, n=1 << 16)
+    for k, other in where.items():
+        over[k] = at[other]
+    ws = over.pop("ws")
+    assert call(ws=ws, **over) == 1
     assert text in L.lib.lssm_last_error().decode()
 
 
