@@ -443,7 +443,8 @@ int lssm_token_logprobs(lssm_ctx* ctx, const void* logits, uint32_t stride, cons
  * stats and entropy (entropy may be NULL without g_entropy; g_logprob,
  * g_entropy NULL: zero):
  *   d_logits[r, v] = g_logprob ([v = t] - p_v) - g_entropy p_v (log p_v + entropy)
- * rounded once.  d_logits may be logits (equal strides). */
+ * rounded once.  d_logits may be logits (equal strides); otherwise no row of one
+ * may overlap one of the other. */
 int lssm_token_logprobs_bwd(lssm_ctx* ctx, const void* logits, uint32_t stride, const int32_t* tokens,
                             const float* stats, const float* entropy, const float* g_logprob,
                             const float* g_entropy, void* d_logits, uint32_t d_stride, uint32_t rows,

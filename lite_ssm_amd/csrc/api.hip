@@ -666,6 +666,20 @@ int logprob_checks(const LogprobArgs& a, int act, const char* name) {
     return LSSM_OK;
 }
 
+// d_logits is logits itself, or none of its rows meets one of theirs (rows
+// of both may take turns in one array)
+int logprob_overlap_check(const LogprobArgs& a, int act, const char* name) {
+    const size_t es = dtype_size(act);
+    const uintptr_t x = (uintptr_t)a.x, d = (uintptr_t)a.dx;
+    LSSM_REQUIRE(x != d || a.stride == a.dx_stride, "%s: in place needs equal strides", name);
+    if (x == d) return LSSM_OK;
+    const size_t nx = ((size_t)(a.rows - 1) * a.stride + a.V) * es, nd = ((size_t)(a.rows - 1) * a.dx_stride + a.V) * es;
+    if (x + nx <= d || d + nd <= x) return LSSM_OK;
+    const size_t pitch = a.stride * es, row = a.V * es, m = (x < d ? d - x : x - d) % pitch;
+    LSSM_REQUIRE(a.stride == a.dx_stride && m >= row && m <= pitch - row, "%s: d_logits overlaps logits", name);
+    return LSSM_OK;
+}
+
 int logprob_ws_check(const LogprobArgs& a, int act, const void* ws, uint64_t ws_bytes, const char* name) {
     if (logprob_segments(a.rows, a.V, act) == 1) return LSSM_OK;
     const size_t need = logprob_ws_bytes(a.rows, a.V, a.K);
@@ -736,7 +750,7 @@ int lssm_token_logprobs_bwd(lssm_ctx* ctx, const void* logits, uint32_t stride, 
     if (int rc = logprob_checks(a, act, name)) return rc;
     LSSM_REQUIRE(d_logits && stats, "%s: null d_logits or stats", name);
     LSSM_REQUIRE(!g_entropy || entropy, "%s: g_entropy needs the entropies", name);
-    LSSM_REQUIRE(d_logits != logits || a.stride == a.dx_stride, "%s: in place needs equal strides", name);
+    if (int rc = logprob_overlap_check(a, act, name)) return rc;
     hipError_t e = launch_logprobs_grad(ctx->stream, a, act);
     if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
     return finish(ctx, name);
@@ -766,8 +780,8 @@ int lssm_token_logprobs_grad(lssm_ctx* ctx, const void* logits, uint32_t stride,
     a.status = ctx->status;
     if (int rc = logprob_checks(a, act, name)) return rc;
     LSSM_REQUIRE(d_logits && stats && entropy, "%s: null d_logits, stats or entropy", name);
-    LSSM_REQUIRE(d_logits != logits || a.stride == a.dx_stride, "%s: in place needs equal strides", name);
     if (int rc = logprob_ws_check(a, act, ws, ws_bytes, name)) return rc;
+    if (int rc = logprob_overlap_check(a, act, name)) return rc;
     hipError_t e = launch_logprobs(ctx->stream, a, act, ws);
     if (e != hipSuccess) return set_error(LSSM_EDEVICE, "%s: %s", name, hipGetErrorString(e));
     return finish(ctx, name);

@@ -373,3 +373,16 @@ def test_a_workspace_for_many_rows_serves_fewer(ctx, V, k):
         want = exact(x[:M], t[:M], k)
         close(lp.cpu(), want[0], 28 * U + 2 * U * want[0].abs(), "logprob")
         assert torch.equal(ids.cpu().long(), want[3])
+
+
+def test_gradient_rows_between_the_logits_rows(ctx):
+    """Rows of logits and of their gradient that take turns in one array."""
+    M, V = 5, 1000
+    x, t = logits(M, V, torch.float16, 9)
+    both = torch.full((M, 2, V), 3.0, dtype=torch.float16, device="cuda")
+    both[:, 0] = x
+    g = torch.ones(M, device="cuda")
+    st, H, want = torch.empty(M, 2, device="cuda"), torch.empty(M, device="cuda"), torch.empty_like(x)
+    ctx.token_logprobs_grad(x, t, g, None, None, H, st, want, M, V, L.F16)
+    ctx.token_logprobs_grad(both, t, g, None, None, H, st, both[0, 1], M, V, L.F16, stride=2 * V, d_stride=2 * V)
+    assert torch.equal(both[:, 0], x) and torch.equal(both[:, 1], want)

@@ -57,6 +57,12 @@ def test_forward_refuses(kw, text):
     (dict(d_stride=99), "row stride"),
     (dict(d=P, logits=P, d_stride=104), "equal strides"),
     (dict(d=2 * P + 1), "not aligned"),
+    (dict(d=P + 2), "overlaps logits"),
+    (dict(d=P + 200), "overlaps logits"),
+    (dict(d=P - 798), "overlaps logits"),
+    (dict(stride=250, d_stride=250, d=P + 198), "overlaps logits"),
+    (dict(stride=250, d_stride=250, d=P + 302), "overlaps logits"),
+    (dict(stride=250, d_stride=249, d=P + 200), "overlaps logits"),
 ])
 def test_backward_refuses(over, text):
     a = dict(logits=P, stride=0, tokens=P, st=P, H=P, g=P, ge=P, d=2 * P, d_stride=0)
