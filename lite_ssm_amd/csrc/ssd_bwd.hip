@@ -62,11 +62,13 @@ constexpr int GP = 32;      // state rows a slice
 constexpr int GXP = 36;     // LDS pitch of a [token][row] tile (= 4 modulo 64 banks x 9)
 constexpr int G_NT = 256;
 
-// slope of dt in raw + bias: the softplus', 0 where the clamp holds
+// slope of dt in v = raw + bias: that of the softplus sp, 0 where the clamp holds
+__device__ __forceinline__ float slope_of(const SsdBwdArgs& a, float v, float sp) {
+    return sp >= a.dt_min && sp <= a.dt_max ? 1.0f / (1.0f + expf(-v)) : 0.0f;
+}
 template <typename T> __device__ __forceinline__ float dt_slope(const SsdBwdArgs& a, uint32_t b, uint32_t t, uint32_t h) {
     const float v = to_f(((const T*)a.dt)[((size_t)b * a.L + t) * a.H + h]) + to_f(((const T*)a.dt_bias)[h]);
-    const float sp = v > 20.0f ? v : log1pf(expf(v));
-    return sp >= a.dt_min && sp <= a.dt_max ? 1.0f / (1.0f + expf(-v)) : 0.0f;
+    return slope_of(a, v, v > 20.0f ? v : log1pf(expf(v)));
 }
 
 struct Steps { double lc, tot; float dt; };
@@ -582,32 +584,54 @@ __device__ __forceinline__ float decay_of(uint32_t t, uint32_t j) {
 __device__ __forceinline__ float nan_of(uint32_t lc) { return lc == LC_NAN ? NAN : 0.0f; }
 
 // dt, the sums of A dt of every chunk and the walks' weights (from the sums in 64
-// bits), zeros and the last sum behind the end: block (chunk, head, sequence), a
-// thread a token
-__global__ __launch_bounds__(FQ) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
-    __shared__ double s[FQ];
-    const uint32_t c = blockIdx.x, h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
+// bits), zeros and the last sum behind the end: a wave a (chunk, head), two
+// tokens a lane; the block's waves take neighbouring heads, whose dt lie
+// together.
+constexpr int ST_W = 4;
+__global__ __launch_bounds__(ST_W * WAVE) void ssd_bwd_steps_kernel(SsdBwdArgs a) {
+    const uint32_t c = blockIdx.x, h = blockIdx.y * ST_W + threadIdx.x / WAVE, b = blockIdx.z, lane = threadIdx.x % WAVE;
+    if (h >= a.H) return;
     const double A = -exp((double)to_f(((const bf16*)a.A_log)[h]));
-    float dt = 0.0f;
-    if (c * FQ + t < a.L) {
-        const float v = to_f(((const bf16*)a.dt)[((size_t)b * a.L + c * FQ + t) * a.H + h]) + to_f(((const bf16*)a.dt_bias)[h]);
-        dt = v > 20.0f ? v : log1pf(expf(v));
-        dt = fminf(fmaxf(dt, a.dt_min), a.dt_max);
+    const float bias = to_f(((const bf16*)a.dt_bias)[h]);
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t uint2v __attribute__((ext_vector_type(2)));
+    f32x2 dt{0.0f, 0.0f}, slope{0.0f, 0.0f}, back, fwd;
+    double s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t t = c * FQ + 2 * lane + k;
+        if (t < a.L) {
+            const float v = to_f(((const bf16*)a.dt)[((size_t)b * a.L + t) * a.H + h]) + bias;
+            const float sp = v > 20.0f ? v : log1pf(expf(v));
+            dt[k] = fminf(fmaxf(sp, a.dt_min), a.dt_max);
+            slope[k] = slope_of(a, v, sp);
+        }
+        s[k] = bounded(A * (double)dt[k]);
     }
-    s[t] = bounded(A * (double)dt);
-    __syncthreads();
-    for (int d = 1; d < FQ; d <<= 1) {
-        const double o = (int)t >= d ? s[t - d] : 0.0;
-        __syncthreads();
-        s[t] += o;
-        __syncthreads();
+    double before = s[0] + s[1];
+#pragma unroll
+    for (int d = 1; d < WAVE; d <<= 1) {
+        const double o = __shfl_up(before, d);
+        if ((int)lane >= d) before += o;
     }
-    const size_t at = (((size_t)b * a.H + h) * a.nchunk + c) * FQ + t;
-    reinterpret_cast<uint32_t*>(a.lc)[at] = to_units(s[t]);
-    a.w_back[at] = expf((float)s[t]);
-    a.w_fwd[at] = dt * expf((float)(s[FQ - 1] - s[t]));
-    a.dtv[at] = dt;
-    a.slope[at] = c * FQ + t < a.L ? dt_slope<bf16>(a, b, c * FQ + t, h) : 0.0f;
+    const double last = __shfl(before, WAVE - 1);
+    before = __shfl_up(before, 1);
+    if (lane == 0) before = 0.0;
+    s[0] += before;
+    s[1] += s[0];
+    uint2v lc;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        lc[k] = to_units(s[k]);
+        back[k] = expf((float)s[k]);
+        fwd[k] = dt[k] * expf((float)(last - s[k]));
+    }
+    const size_t at = (((size_t)b * a.H + h) * a.nchunk + c) * FQ + 2 * lane;
+    *reinterpret_cast<uint2v*>(a.lc + at) = lc;
+    *reinterpret_cast<f32x2*>(a.dtv + at) = dt;
+    *reinterpret_cast<f32x2*>(a.slope + at) = slope;
+    *reinterpret_cast<f32x2*>(a.w_back + at) = back;
+    *reinterpret_cast<f32x2*>(a.w_fwd + at) = fwd;
 }
 
 // where tile (row tile, column tile) of a kept state's piece starts
@@ -1396,7 +1420,7 @@ hipError_t launch_ssd_bwd(hipStream_t s, SsdBwdArgs a, const lssm_ssd_dims& d, i
         using T = decltype(z);
         if (a.batch) {
             if (fast) {
-                if (a.nchunk) ssd_bwd_steps_kernel<<<dim3(a.nchunk, a.H, a.batch), FQ, 0, s>>>(a);
+                if (a.nchunk) ssd_bwd_steps_kernel<<<dim3(a.nchunk, (a.H + ST_W - 1) / ST_W, a.batch), ST_W * WAVE, 0, s>>>(a);
                 ssd_bwd_walk_bf16_kernel<<<dim3(a.H * a.nslice * (FN / NC), a.batch, 2), W_NT, 0, s>>>(a);
                 if (a.nchunk)
                     ssd_bwd_chunk_bf16_kernel<<<dim3(a.nchunk * a.nsplit * a.G, a.batch), F_NT, 0, s>>>(a);
