@@ -646,7 +646,7 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // once is contiguous (32 bytes of each of four waves to a line stored at 3.0
 // TB/s), and a lane of the chunks' kernel finds its operand in 16 bytes.
 constexpr int W_NT = 256, NC = 64;
-__global__ __launch_bounds__(W_NT, 4) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
+__global__ __launch_bounds__(W_NT, 3) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
     constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 16;
     constexpr int XV = FQ * FP / 8 / W_NT, BV = FQ * NC / 8 / W_NT;     // 16-byte pieces a thread stages
     __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * BP];
