@@ -10,8 +10,11 @@
 //
 // A block reads one segment of a row into registers, once: all of its loads
 // are in flight together, and the maximum, the sums, the alternatives and the
-// gradient are passes over registers.  A row of more than LP_MAXV vectors, or
-// one of few rows, is cut into segments that a second launch joins.
+// gradient are passes over registers.  A row that does not fit one block's
+// registers, or one of few rows, is cut into segments that a second launch
+// joins.  Bound: the logits' bytes (8000 x 50280 bf16: 182 us, 4.4 TB/s; with the
+// gradient 2048 x 50280: 94 us, 4.4 TB/s read and written); with few rows the
+// latency of the load, the passes and the launches.
 //
 // Masked logits: -inf has p = 0 and adds nothing (p log p is 0 there);
 // the type's lowest value is an ordinary number.  A row with nothing but -inf
@@ -166,7 +169,11 @@ template <typename T> struct RowSpan {
     }
 };
 
-// One segment of a row (the whole row where a.S == 1).
+// One segment of a row (the whole row where a.S == 1).  Alternatives: a value no
+// less than K of the block's is found from the lanes' maxima, what lies above it
+// is collected (a K or two) and ranked.  They cost 3 us with K = 1 and 6 with
+// 64 (1 x 50280: 6.1 us without, 9.2 to 12.3 with), most of it the search's serial
+// steps; a second pass over the logits is never needed.
 // GRAD (a.S == 1, no alternatives): the gradient is written from the registers too.
 template <typename T, int R, bool GRAD, int LP_NT>
 __global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {
@@ -394,7 +401,9 @@ __global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {
     }
 }
 
-// Joins a row's segments: the sums, then the best of the segments' best.
+// Joins a row's segments: the sums, then the best of the segments' best.  A
+// block a row, one wave for the sums; latency only (2.4 us without alternatives,
+// 4 to 5 with 20).
 template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a) {
     const uint32_t r = blockIdx.x, tid = threadIdx.x, S = a.S, K = a.K;
     const float* p = a.part + 3 * (size_t)r * S;
@@ -457,7 +466,11 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
     }
 }
 
-// The gradient from kept statistics: one pass, a block a stretch of a row.
+// The gradient from kept statistics: one pass, a block a stretch of a row of
+// LG_R vectors a thread, a read and a write of 16 bytes apiece; bound by them
+// (700 x 256000 bf16: 121 us, 5.9 TB/s with the logits partly in the last-level
+// cache; splitting the rows so that more of them stay there measured no faster:
+// 217 us for loss and gradient at once, 226 in two, 275 in five).
 constexpr int LG_NT = 256, LG_R = 4;
 template <typename T> __global__ __launch_bounds__(LG_NT) void logprob_grad_kernel(LogprobArgs a) {
     constexpr int E = Vec<T>::E;
@@ -521,26 +534,33 @@ template <typename F> hipError_t with_type(int act, F f) {
 
 }  // namespace
 
-// How a row is cut: segments, threads a block, 16-byte vectors a thread.
-// Blocks of LP_WIDE threads, a segment as long as their registers hold; where
-// these are fewer than LP_FEW, blocks of LP_SMALL threads, as many as LP_WANT
-// allows (us, wide -> small, bf16, alternatives): 1 x 50280, 5: 11.5 -> 9.3;
-// 8 x 50280, 5: 12.4 -> 9.8; 1 x 256000, 20: 16.6 -> 14.8; 32 x 50280, 20:
-// 12.4 both; 64 x 50280, none: 7.2 -> 8.4; 128 x 50280, 5: 11.9 -> 14.3.
-// LP_WANT 256 and 1024 measured alike.
+// How a row is cut: segments, threads a block, 16-byte vectors a thread (the
+// least that hold a segment: 4096 rows of 8000 take 36 us so, 79 at 8).
+//   - A row that LP_SMALL threads hold is one segment of theirs: 4096 rows, bf16,
+//     of LP_WIDE -> of LP_SMALL threads: 2000 logits 33.6 -> 10.6 us, 8000 35.1
+//     -> 18.3, 16000 37.1 -> 28.5 (loss and gradient 61.1 -> 55.3).
+//   - A longer one is cut for LP_WIDE threads, a segment as long as LP_MAXR
+//     vectors allow: 2048 x 50280 in one pass of 93.8 us with its gradient, cut
+//     in two (LP_MAXR 4) 130; 8000 x 50280 with 5 alternatives 215 and 294.
+//   - Where all this makes fewer than LP_FEW blocks, it is cut finer, for
+//     LP_SMALL threads, as far as LP_WANT blocks go: 1 x 50280 with 5
+//     alternatives 11.5 -> 9.3, 8 rows of those 12.4 -> 9.8, 1 x 256000 with 20
+//     16.6 -> 14.8; 32 x 50280 with 20 12.4 both, 64 without any 7.2 -> 8.4, 128
+//     with 5 11.9 -> 14.3.  (LP_WANT 256 and 1024 measured alike.)
 constexpr uint32_t LP_FEW = 32, LP_WANT = 512;
 struct LogprobPlan { uint32_t S, nt, R; };
 static LogprobPlan plan_of(uint32_t rows, uint32_t vocab, int act) {
     const uint32_t nv = std::max(1u, vocab / (act == LSSM_F32 ? 4u : 8u));
     auto segs = [&](uint32_t nt, uint32_t R) { return (nv + nt * R - 1) / (nt * R); };
     const uint32_t S = segs(LP_WIDE, LP_MAXR);
+    uint32_t R = 2;
     if ((uint64_t)rows * S < LP_FEW && segs(LP_SMALL, LP_MAXR) <= LP_MAXS) {
-        uint32_t R = 2;
         while (R < LP_MAXR && (rows * segs(LP_SMALL, R) > LP_WANT || segs(LP_SMALL, R) > LP_MAXS)) R *= 2;
         return {segs(LP_SMALL, R), LP_SMALL, R};
     }
-    const uint32_t per = (nv + S - 1) / S;
-    return {S, LP_WIDE, per <= 2 * LP_WIDE ? 2u : per <= 4 * LP_WIDE ? 4u : 8u};
+    const uint32_t nt = nv <= LP_SMALL * LP_MAXR ? LP_SMALL : LP_WIDE;
+    while (R < LP_MAXR && segs(nt, R) > S) R *= 2;
+    return {S, nt, R};
 }
 
 uint32_t logprob_segments(uint32_t rows, uint32_t vocab, int act) { return plan_of(rows, vocab, act).S; }
@@ -575,15 +595,21 @@ hipError_t launch_logprobs(hipStream_t s, LogprobArgs a, int act, void* ws) {
         using T = decltype(z);
         const dim3 grid(a.rows * a.S);
         const bool grad = a.dx && a.S == 1;
-        auto go = [&](auto rc) {
-            constexpr int R = decltype(rc)::value;
-            if (p.nt == LP_SMALL && !grad) logprob_seg_kernel<T, R, false, LP_SMALL><<<grid, LP_SMALL, 0, s>>>(a);
-            else if (grad) logprob_seg_kernel<T, R, true, LP_WIDE><<<grid, LP_WIDE, 0, s>>>(a);
-            else logprob_seg_kernel<T, R, false, LP_WIDE><<<grid, LP_WIDE, 0, s>>>(a);
+        auto go = [&](auto rc, auto ntc) {
+            constexpr int R = decltype(rc)::value, NT = decltype(ntc)::value;
+            if (grad) logprob_seg_kernel<T, R, true, NT><<<grid, NT, 0, s>>>(a);
+            else logprob_seg_kernel<T, R, false, NT><<<grid, NT, 0, s>>>(a);
         };
-        if (p.R == 2) go(std::integral_constant<int, 2>{});
-        else if (p.R == 4) go(std::integral_constant<int, 4>{});
-        else go(std::integral_constant<int, 8>{});
+        constexpr std::integral_constant<int, LP_SMALL> small;
+        constexpr std::integral_constant<int, LP_WIDE> wide;      // (rows of more than LP_SMALL 8 vectors: R 4 or 8)
+        if (p.nt == LP_SMALL) {
+            if (p.R == 2) go(std::integral_constant<int, 2>{}, small);
+            else if (p.R == 4) go(std::integral_constant<int, 4>{}, small);
+            else go(std::integral_constant<int, 8>{}, small);
+        } else {
+            if (p.R <= 4) go(std::integral_constant<int, 4>{}, wide);
+            else go(std::integral_constant<int, 8>{}, wide);
+        }
         if (a.S > 1) logprob_join_kernel<T><<<a.rows, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !a.dx || grad) return e;
