@@ -29,6 +29,13 @@
 // Three steps: the states h0 (forwards) and G1 (backwards) of every chunk are
 // kept; the chunks' gradients, in parallel; sums over heads, slices and chunks.
 // Every order of summation is fixed.
+//
+// Two forms.  The bf16 one (second half of this file) takes bf16 with N = 128, P
+// in 64s and 16-byte aligned arrays, the generic one everything else.  Us,
+// generic -> bf16 form, same inputs: a 130M layer (24 heads) of 37 tokens 34.1 ->
+// 34.6, 128 40.0 -> 35.8, 512 62.8 -> 47.0, 2048 150 -> 76; a 2.7B layer (80 heads)
+// of 37 tokens 61 -> 44, 4096 951 -> 241, 4 x 4096 3842 -> 722.  (At one token of 24
+// heads the generic form is 3 us faster; no rule is made for that.)
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -164,7 +171,10 @@ template <typename T, int W, int NTH> __device__ __forceinline__ void load_tile(
 
 // What a chunk alone adds to the state behind it (direction 0: weighted outer
 // products of x with B) or to the gradient in front of it (1: of dy with C):
-// block (head, slice and direction; chunk; sequence).
+// block (head, slice and direction; chunk; sequence).  Bound by the states it
+// writes; 512 tokens of 24 heads in fp32: 13 us.  (With a walk over the chunks
+// instead of this and the scan, states in registers, all launches took 232 us
+// there, and 88 so.)
 template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_own_kernel(SsdBwdArgs a) {
     constexpr int NP = NT + 4, TN = NT / 64;
     __shared__ __attribute__((aligned(16))) float Rs[GQ * GXP], Cs[GQ * NP], W[GQ];
@@ -207,7 +217,8 @@ template <typename T, int NT> __global__ __launch_bounds__(G_NT) void ssd_bwd_ow
 
 // The scan: an element of a head's state a thread.  Slot c holds what chunk c
 // adds and gets the state that enters it (direction 0), or the gradient of the
-// one that leaves it (1).  Slots are read SC ahead.
+// one that leaves it (1).  Slots are read SC ahead; bound by reading and writing
+// them (10 us at 512 tokens of 24 heads).
 constexpr int SC = 8;
 __global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
     const uint32_t PN = a.P * a.N, i = blockIdx.x / 2 * G_NT + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
@@ -242,6 +253,10 @@ __global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
 // T0, rows J0); eight waves split the k of dx over the state's columns.  The
 // next pair's rows and states are on their way into registers meanwhile, where
 // they can be taken 16 bytes at a time.  Two blocks fit a CU up to N = 128.
+// Bound by latency and fp32 MFMA issue: 50 us at 512 tokens of 24 heads.  Eight
+// waves with the prefetch against four without: 4096 tokens of 80 heads 1519 ->
+// 1104 us, N = 200 3461 -> 1831; two blocks a CU: 1104 -> 975, 1831 -> 1430.  N <= 64
+// has too few columns for eight waves.
 template <typename T, int NT, int NW> __global__ __launch_bounds__(64 * NW, NT == 256 ? 2 : 4) void ssd_bwd_chunk_kernel(SsdBwdArgs a) {
     constexpr int NP = NT + 4, TN = NT / (16 * NW), NTH = 64 * NW, KG = NW / 4;
     __shared__ __attribute__((aligned(16))) float Bs[GQ * NP], Hs[GP * NP], Gs[GP * NP];
@@ -643,8 +658,13 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // direction; wave w keeps the state's rows 16 w .. + 15, all NC columns of the
 // part, in fp32.  A chunk's state goes out as two pieces, in tiles of 16 rows by
 // 16 columns ([row tile][column tile][piece][n][row]): what a wave stores at
-// once is contiguous (32 bytes of each of four waves to a line stored at 3.0
-// TB/s), and a lane of the chunks' kernel finds its operand in 16 bytes.
+// once is contiguous (32 bytes of each of four waves to a line: 424 us where this
+// takes 333, 4 x 4096 tokens), and a lane of the chunks' kernel finds its operand
+// in 16 bytes.  A walk of 32 steps is latency at one sequence (111 us at 4096
+// tokens, 320 blocks on 256 CUs: the waves issue 41 % of their cycles and wait for
+// memory or LDS 24 %), and bandwidth and issue at four (310 us: 1.07 GB, 3.4
+// TB/s).  NC 32, 64, 128: 93, 86, 97 us at one sequence with the inputs in cache,
+// 409, 300, 300 at four.
 constexpr int W_NT = 256, NC = 64;
 __global__ __launch_bounds__(W_NT, 3) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
     constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 16;
@@ -784,6 +804,12 @@ __global__ __launch_bounds__(W_NT, 3) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
 // C B^T and the heads' sum of S (lower tiles, as their product leaves them) live
 // in LDS.  The next pair's rows and states are on their way into registers
 // while this one is worked on.
+// Bound by its own instructions: 120 us at 4096 tokens of 80 heads, of which 115
+// stay when all loads come from the caches.  A wave issues 1256 VALU, 141 MFMA
+// and 217 LDS instructions a pair (VALU 45 % of the SIMDs' cycles, MFMA 20 %), and
+// the wave of source tile 0 has eight dependent tiles of S in a row.  Two tiles
+// at a time need more than the 256 registers that two waves a SIMD leave: 213 us
+// with their spills.
 constexpr int F_TILES = 36;
 __device__ __forceinline__ constexpr int tile_of(int T, int J) { return T * (T + 1) / 2 + J; }
 
@@ -1342,7 +1368,8 @@ Plan plan_of(uint32_t batch, const lssm_ssd_dims& d, bool fast) {
     p.nchunk = (d.L + qn - 1) / qn;
     p.nslice = (d.P + rn - 1) / rn;
     // shares of a group's (head, slice) pairs: the fewest rounds of blocks
-    // over the chip, a block's own work taken as two pairs more
+    // over the chip, a block's own work taken as two pairs more (as none: 16
+    // heads of N = 64, 2 x 1777 tokens 125 -> 147 us; as six: all alike)
     const uint32_t pairs = d.H / d.n_groups * p.nslice;
     const size_t blocks = std::max<size_t>(1, (size_t)p.nchunk * batch * d.n_groups), cus = (fast ? 1 : 2) * (size_t)num_cus();
     size_t best = 0;
