@@ -662,17 +662,21 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // takes 333, 4 x 4096 tokens), and a lane of the chunks' kernel finds its operand
 // in 16 bytes.  A walk of 32 steps is latency at one sequence (111 us at 4096
 // tokens, 320 blocks on 256 CUs: the waves issue 41 % of their cycles and wait for
-// memory or LDS 24 %), and bandwidth and issue at four (310 us: 1.07 GB, 3.4
-// TB/s).  NC 32, 64, 128: 93, 86, 97 us at one sequence with the inputs in cache,
+// memory or LDS 24 %), and bandwidth and issue at four (296 us: 0.89 GB, 3.0
+// TB/s; 310 us with the parts of a slice on two XCDs, which read its rows twice).  NC 32, 64, 128: 93, 86, 97 us at one sequence with the inputs in cache,
 // 409, 300, 300 at four.
 constexpr int W_NT = 256, NC = 64;
+constexpr uint32_t XCDS = 8;
 __global__ __launch_bounds__(W_NT, 3) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a) {
     constexpr int PARTS = FN / NC, NTL = NC / 16, BP = NC + 16;
     constexpr int XV = FQ * FP / 8 / W_NT, BV = FQ * NC / 8 / W_NT;     // 16-byte pieces a thread stages
     __shared__ __attribute__((aligned(16))) bf16 Xs[FQ * FXP], Bs[FQ * BP];
     __shared__ __attribute__((aligned(16))) float W[FQ];
-    const uint32_t n0 = blockIdx.x % PARTS * NC, h = blockIdx.x / PARTS / a.nslice, sl = blockIdx.x / PARTS % a.nslice;
-    const uint32_t b = blockIdx.y;
+    // The parts of a head's slice read the same rows: they are XCDS blocks apart,
+    // which one XCD gets, and its L2 serves the second.
+    const uint32_t all = a.H * a.nslice, first = blockIdx.x / (XCDS * PARTS) * XCDS, some = min(XCDS, all - first);
+    const uint32_t at8 = blockIdx.x - first * PARTS, n0 = at8 / some * NC, hs = first + at8 % some;
+    const uint32_t h = hs / a.nslice, sl = hs % a.nslice, b = blockIdx.y;
     const bool back = blockIdx.z != 0;
     const uint32_t P = a.P, L = a.L, g = h / (a.H / a.G), tid = threadIdx.x;
     const int lane = tid % WAVE, li = lane % 16, lq = lane / 16, tk = li / 4, tc = li % 4;
