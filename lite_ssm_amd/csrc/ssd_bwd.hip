@@ -253,7 +253,7 @@ __global__ __launch_bounds__(G_NT) void ssd_bwd_scan_kernel(SsdBwdArgs a) {
 // T0, rows J0); eight waves split the k of dx over the state's columns.  The
 // next pair's rows and states are on their way into registers meanwhile, where
 // they can be taken 16 bytes at a time.  Two blocks fit a CU up to N = 128.
-// Bound by latency and fp32 MFMA issue: 50 us at 512 tokens of 24 heads.  Eight
+// Bound by latency and fp32 MFMA issue: 37 us at 512 tokens of 24 heads.  Eight
 // waves with the prefetch against four without: 4096 tokens of 80 heads 1519 ->
 // 1104 us, N = 200 3461 -> 1831; two blocks a CU: 1104 -> 975, 1831 -> 1430.  N <= 64
 // has too few columns for eight waves.
@@ -662,7 +662,7 @@ __device__ __forceinline__ constexpr uint32_t state_at(uint32_t pt, uint32_t nt,
 // takes 333, 4 x 4096 tokens), and a lane of the chunks' kernel finds its operand
 // in 16 bytes.  A walk of 32 steps is latency at one sequence (111 us at 4096
 // tokens, 320 blocks on 256 CUs: the waves issue 41 % of their cycles and wait for
-// memory or LDS 24 %), and bandwidth and issue at four (296 us: 0.89 GB, 3.0
+// memory or LDS 24 %), and bandwidth and issue at four (296 us: 1.25 GB, 4.2
 // TB/s; 310 us with the parts of a slice on two XCDs, which read its rows twice).  NC 32, 64, 128: 93, 86, 97 us at one sequence with the inputs in cache,
 // 409, 300, 300 at four.
 constexpr int W_NT = 256, NC = 64;
