@@ -88,6 +88,37 @@ def test_engine_scores_a_prompt(ctx, act, wfmt, B, n, vocab):
     eng.close()
 
 
+@pytest.mark.parametrize("B,n", [(2, 4096), (1, 8192)])
+def test_a_prefill_of_two_halves_is_scored(ctx, B, n):
+    """8192 rows run as two halves on two streams (batch, or time), with a trace
+    buffer set as one.  The two forms' logits are each within 2e-2 of the largest
+    of the reference's, so their log probabilities within 8e-2 of it; a row
+    that is not its position's is off by several units."""
+    sh = shape("mamba2-130m", n_layer=2, vocab_size=1024)
+    m = DeviceModel(sh, act=L.BF16, wfmt=L.W_Q4_G64, seed=3, embed_std=0.1)
+    torch.cuda.synchronize()
+    eng = Engine(ctx, m, max_batch=B, max_seq=n)
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(0, 1024, (B, n), generator=g, dtype=torch.int32).cuda()
+    nxt = torch.zeros(B, dtype=torch.int32, device="cuda")
+    lp, H = ([torch.full((B, n), 7.0, device="cuda") for _ in range(2)] for _ in range(2))
+    top, tlp = torch.zeros(B, n, 1, dtype=torch.int32, device="cuda"), torch.zeros(B, n, 1, device="cuda")
+    eng.score(ids, nxt, ids, lp[0], H[0], top, tlp)
+    torch.cuda.synchronize()
+    assert torch.equal(top[:, -1, 0], nxt)
+    trace = torch.zeros((sh.n_layer + 1) * B * n, sh.d_model, dtype=torch.bfloat16, device="cuda")
+    eng.set_trace(trace)
+    eng.reset()
+    eng.score(ids, nxt, ids, lp[1], H[1])
+    torch.cuda.synchronize()
+    given, entropy, all_lp, err = expected(m, trace[sh.n_layer * B * n:], ids.reshape(-1))
+    assert bool(((lp[1].reshape(-1).double() - given).abs() <= err).all())
+    largest = float((all_lp - all_lp.mean(-1, keepdim=True)).abs().max())
+    assert float((lp[0] - lp[1]).abs().max()) <= 8e-2 * largest < 2.0
+    eng.set_trace(None)
+    eng.close()
+
+
 def test_engine_score_refuses(ctx):
     sh = shape("mamba2-130m", n_layer=1, vocab_size=128)
     m = DeviceModel(sh, act=L.BF16, wfmt=L.W_Q4_G64, seed=3)

@@ -96,6 +96,17 @@ def test_sizes(ctx, act, H, P, G, N):
     check(call(ctx, v, code), v, dt)
 
 
+# several chunks, slices and groups at once, head counts around those that share
+# an XCD or a block
+@pytest.mark.parametrize("act", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("b,n,H,P,G,N", [(2, 400, 12, 64, 3, 128), (1, 700, 5, 128, 1, 128), (3, 130, 9, 192, 9, 128),
+                                         (2, 333, 7, 40, 7, 100), (1, 513, 24, 64, 1, 64)])
+def test_many_chunks_slices_and_groups(ctx, act, b, n, H, P, G, N):
+    code, dt = ACT[act]
+    v = inputs(dt, b, n, H, P, G, N, 17 * n + H)
+    check(call(ctx, v, code), v, dt)
+
+
 @pytest.mark.parametrize("act", ["f32", "bf16", "f16"])
 def test_no_states_no_D(ctx, act):
     code, dt = ACT[act]
@@ -254,3 +265,29 @@ def test_against_differences(ctx):
     names = dict(X="dX", B="dB", C="dC", dt="d_dt", state="d_state0")
     want = sum(float((got[names[k]].double() * way[k].double()).sum()) for k in way)
     assert abs(num - want) < 1e-2 * max(1.0, abs(want)), (num, want)
+
+
+def test_two_contexts_at_once(ctx):
+    """Two streams, a workspace each, calls in turn without waiting."""
+    cases = [("bf16", inputs(torch.bfloat16, 1, 500, 8, 64, 1, 128, 51)), ("f32", inputs(torch.float32, 2, 200, 4, 64, 2, 128, 52))]
+    want = [call(ctx, v, ACT[a][0]) for a, v in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    ctxs = [L.Ctx(stream=s.cuda_stream) for s in streams]
+    runs = []
+    for c, (a, v) in zip(ctxs, cases):
+        t, o, d = {k: x.cuda() for k, x in v.items()}, outputs(v), dims(v)
+        runs.append((c, t, o, d, workspace(c, v, d, ACT[a][0])[1], ACT[a][0], v["X"].shape[0]))
+    torch.cuda.synchronize()
+    for c in ctxs:
+        c.begin_batch()
+    for _ in range(20):
+        for c, t, o, d, ws, code, b in runs:
+            c.ssd_chunked_bwd(t["X"], t["B"], t["C"], t["dt"], t["dt_bias"], t["A_log"], t["D"], t["state"], t["dY"],
+                              t["d_state"], o["dX"], o["dB"], o["dC"], o["d_dt"], o["d_dt_bias"], o["dA_log"], o["dD"],
+                              o["d_state0"], b, d, code, ws)
+    for c in ctxs:
+        c.commit_and_wait()
+    for (c, t, o, *_), w in zip(runs, want):
+        for k in w:
+            assert torch.equal(o[k].cpu(), w[k]), k
+        c.close()
