@@ -255,12 +255,13 @@ __global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {
         // Two values that at least K of the block's are no less than: the K-th
         // best of a wave's lanes' best values, and the lowest of the waves'
         // ceil(K / waves)-th best ones.  Either may be the larger.  Found bit
-        // by bit, down to bits 12 (a 2^-11-th below them at most, which only
-        // lengthens the list).
+        // by bit, down to the last that a 16-bit logit has, or to 2^-13 of fp32's
+        // (lower ones would only shorten the list).
+        constexpr int last = sizeof(T) == 4 ? 10 : (__is_same(T, bf16) ? 16 : 13);
         constexpr uint32_t nw = LP_NW;
         const uint32_t best = ord_of(m), K2 = (K + nw - 1) / nw;
         uint32_t tau = 0, tau2 = 0;
-        for (int bit = 31; bit >= 12; --bit) {
+        for (int bit = 31; bit >= last; --bit) {
             const uint32_t c = tau | (1u << bit), c2 = tau2 | (1u << bit);
             if ((uint32_t)__popcll(__ballot(best >= c)) >= K) tau = c;
             if ((uint32_t)__popcll(__ballot(best >= c2)) >= K2) tau2 = c2;
@@ -406,6 +407,20 @@ __global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {
 // 4 to 5 with 20).
 template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel(LogprobArgs a) {
     const uint32_t r = blockIdx.x, tid = threadIdx.x, S = a.S, K = a.K;
+    // all first loads at once
+    const u64* in = a.part_keys + (size_t)r * S * K;
+    const u64 mine = tid < S * K ? in[tid] : 0;
+    u64 head = 0, late = 0;
+    if (K && tid < S) {
+        head = in[(size_t)tid * K];
+        late = in[(size_t)tid * K + (K + S - 1) / S - 1];
+    }
+    int t = -1;
+    float xt = 0.0f;
+    if (tid == 0 && a.tokens) {
+        t = a.tokens[r];
+        if (t >= 0 && (uint32_t)t < a.V) xt = to_f(((const T*)a.x)[(size_t)r * a.stride + t]);
+    }
     const float* p = a.part + 3 * (size_t)r * S;
     Soft s{-FLT_MAX, 0.0f, 0.0f};
     for (uint32_t i = tid % WAVE; i < S; i += WAVE) {
@@ -419,11 +434,7 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
     s.T = wave_sum(s.T);
     s = same(s);
     const RowOut o = row_out(s);
-    if (tid == 0) {
-        const int t = a.tokens ? a.tokens[r] : -1;
-        const T* row = (const T*)a.x + (size_t)r * a.stride;
-        store_row(a, r, o, t >= 0 && (uint32_t)t < a.V ? to_f(row[t]) : 0.0f, t);
-    }
+    if (tid == 0) store_row(a, r, o, xt, t);
     if (K == 0) return;
     // A segment's keys are in order: the i-th of the segment whose best has
     // rank h among the segments' is behind i of its own and h others, so only
@@ -431,16 +442,15 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
     // below the lowest of all segments' ceil(K / S)-th keys.
     __shared__ u64 keys[LP_JOIN];
     __shared__ uint32_t rank[LP_MAXS], count, found;
-    const u64* in = a.part_keys + (size_t)r * S * K;
     if (tid < S) {
-        keys[tid] = in[(size_t)tid * K];
-        keys[LP_MAXS + tid] = in[(size_t)tid * K + (K + S - 1) / S - 1];
+        keys[tid] = head;
+        keys[LP_MAXS + tid] = late;
     }
     if (tid == 0) count = found = 0;
     __syncthreads();
     if (tid < S) {
         uint32_t h = 0;
-        for (uint32_t j = 0; j < S; ++j) h += keys[j] > keys[tid] ? 1u : 0u;
+        for (uint32_t j = 0; j < S; ++j) h += keys[j] > head ? 1u : 0u;
         rank[tid] = h;
     }
     u64 least = ~0ull;
@@ -449,7 +459,7 @@ template <typename T> __global__ __launch_bounds__(256) void logprob_join_kernel
     for (uint32_t i = tid; i < S * K; i += 256) {
         const uint32_t sg = i / K;
         if (rank[sg] + (i - sg * K) < K) {
-            const u64 k = in[i];
+            const u64 k = i == tid ? mine : in[i];
             if (k && k >= least) keys[atomicAdd(&count, 1u)] = k;      // 0: an empty place
         }
     }
