@@ -35,7 +35,7 @@ namespace {
 constexpr uint32_t LP_MAXR = 8;              // 16-byte vectors a thread holds
 constexpr uint32_t LP_WIDE = 1024, LP_SMALL = 256;   // threads of a segment's block
 constexpr int LP_CAP = 1024;                 // candidates of a segment's alternatives
-constexpr uint32_t LP_MAXS = 64;             // segments of a row
+constexpr uint32_t LP_MAXS = 128;             // segments of a row
 constexpr int LP_JOIN = LSSM_LOGPROB_MAX_TOP * (LSSM_LOGPROB_MAX_TOP + 1) / 2;
 static_assert(LSSM_LOGPROB_MAX_VOCAB / 4 <= LP_MAXS * LP_WIDE * LP_MAXR, "segments");
 static_assert(LP_JOIN % 8 == 0 && LP_CAP % 8 == 0, "lists");
@@ -557,7 +557,10 @@ template <typename F> hipError_t with_type(int act, F f) {
 //     alternatives 11.5 -> 9.3, 8 rows of those 12.4 -> 9.8, 1 x 256000 with 20
 //     16.6 -> 14.8; 32 x 50280 with 20 12.4 both, 64 without any 7.2 -> 8.4, 128
 //     with 5 11.9 -> 14.3.  (LP_WANT 256 and 1024 measured alike.)
-constexpr uint32_t LP_FEW = 32, LP_WANT = 512;
+//   - Rows of several segments that make LP_HALF blocks at most, half the CUs,
+//     are cut in twice as many: 10 x 256000 with 20 alternatives 16.6 -> 14.0, 32 of
+//     those 17.4 -> 15.6; 50 of them 18.2 -> 19.9.
+constexpr uint32_t LP_FEW = 32, LP_HALF = 128, LP_WANT = 512;
 struct LogprobPlan { uint32_t S, nt, R; };
 static LogprobPlan plan_of(uint32_t rows, uint32_t vocab, int act) {
     const uint32_t nv = std::max(1u, vocab / (act == LSSM_F32 ? 4u : 8u));
@@ -569,6 +572,7 @@ static LogprobPlan plan_of(uint32_t rows, uint32_t vocab, int act) {
         return {segs(LP_SMALL, R), LP_SMALL, R};
     }
     const uint32_t nt = nv <= LP_SMALL * LP_MAXR ? LP_SMALL : LP_WIDE;
+    if (S > 1 && (uint64_t)rows * S <= LP_HALF) return {segs(LP_WIDE, LP_MAXR / 2), LP_WIDE, LP_MAXR / 2};
     while (R < LP_MAXR && segs(nt, R) > S) R *= 2;
     return {S, nt, R};
 }
@@ -587,7 +591,7 @@ size_t logprob_ws_bytes(uint32_t rows, uint32_t vocab, uint32_t top_k) {
             if (S > 1) n = std::max(n, part_bytes(r, S) + (size_t)r * S * top_k * 8);
         }
     };
-    for (uint32_t r = 1; r < std::min(rows, LP_FEW); ++r) of(r);
+    for (uint32_t r = 1; r < std::min(rows, LP_HALF + 1); ++r) of(r);
     of(rows);
     return n;
 }

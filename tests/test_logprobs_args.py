@@ -99,5 +99,5 @@ def test_workspace_grows_with_what_it_holds():
 @pytest.mark.parametrize("k", [0, 5, 64])
 @pytest.mark.parametrize("V", [100, 2049, 50280, 65544, 256000, 2097152])
 def test_workspace_of_some_rows_is_enough_for_fewer(V, k):
-    sizes = [L.lib.lssm_token_logprobs_workspace(r, V, k) for r in range(1, 80)]
+    sizes = [L.lib.lssm_token_logprobs_workspace(r, V, k) for r in range(1, 140)]
     assert sizes == sorted(sizes)
