@@ -171,9 +171,10 @@ template <typename T> struct RowSpan {
 
 // One segment of a row (the whole row where a.S == 1).  Alternatives: a value no
 // less than K of the block's is found from the lanes' maxima, what lies above it
-// is collected (a K or two) and ranked.  They cost 3 us with K = 1 and 6 with
-// 64 (1 x 50280: 6.1 us without, 9.2 to 12.3 with), most of it the search's serial
-// steps; a second pass over the logits is never needed.
+// is collected (a K or two) and ranked.  They cost 1.6 us with K = 1 and 5
+// with 64 in a block of few rows (1 x 50280: 3.1 us without, 4.7 and 8.3 with), 3
+// and 6 in a block of LP_WIDE threads; only more equal values than the list
+// holds take further passes, over the registers.
 // GRAD (a.S == 1, no alternatives): the gradient is written from the registers too.
 template <typename T, int R, bool GRAD, int LP_NT>
 __global__ __launch_bounds__(LP_NT, 8) void logprob_seg_kernel(LogprobArgs a) {

@@ -808,12 +808,14 @@ __global__ __launch_bounds__(W_NT, 3) void ssd_bwd_walk_bf16_kernel(SsdBwdArgs a
 // C B^T and the heads' sum of S (lower tiles, as their product leaves them) live
 // in LDS.  The next pair's rows and states are on their way into registers
 // while this one is worked on.
-// Bound by its own instructions: 120 us at 4096 tokens of 80 heads, of which 115
-// stay when all loads come from the caches.  A wave issues 1256 VALU, 141 MFMA
-// and 217 LDS instructions a pair (VALU 45 % of the SIMDs' cycles, MFMA 20 %), and
-// the wave of source tile 0 has eight dependent tiles of S in a row.  Two tiles
-// at a time need more than the 256 registers that two waves a SIMD leave: 213 us
-// with their spills.
+// No one thing bounds it: 450 us at 4 x 4096 tokens of 80 heads; 394 with all
+// loads from the caches, 392 without S and M, 420 without dx' from G1, 441 without
+// dC of what was before the chunk, and 194 with none of these and no dB: staging,
+// barriers and dx in a row.  A wave issues 1256 VALU, 141 MFMA and 217 LDS
+// instructions a pair (VALU 45 % of the SIMDs' cycles, MFMA 20 %).  Two tiles of S
+// at a time need more than the 256 registers that two waves a SIMD leave (120 ->
+// 213 us at 4096 tokens, with spills); the next pair's rows fetched before S, and
+// B and h0 at the pair's start instead, came out even (457 and 464).
 constexpr int F_TILES = 36;
 __device__ __forceinline__ constexpr int tile_of(int T, int J) { return T * (T + 1) / 2 + J; }
 
